@@ -86,19 +86,23 @@ def build(verbose=False, force=False, ptxas_info=False):
         if os.path.exists(GEMM_AR):
             os.remove(GEMM_AR)
         subprocess.check_call(["ar", "rcs", GEMM_AR] + gemm_objs)
-    # the loss drop-in (fused softmax cross-entropy): its own shared + static library, no dependency on the attention engine
-    loss_src = os.path.join(HERE, "loss", "cross_entropy.cu")
-    loss_obj = os.path.join(OBJDIR, "cross_entropy.o")
-    loss_deps = [loss_src, os.path.join(CSRC, "tc_common.cuh"), os.path.join(HERE, "..", "include", "kernels", "loss.cuh"),
-                 os.path.join(HERE, "..", "include", "b200loss.h")]
-    if force or _stale(loss_obj, loss_deps):
-        subprocess.check_call([nvcc] + ARCH + FLAGS + ["-I", os.path.join(HERE, "..", "include"), "-I", CSRC, "-c", loss_src, "-o", loss_obj])
-    if force or _stale(LOSS_SO, [loss_obj]):
-        subprocess.check_call([nvcc] + ARCH + ["-shared", "-o", LOSS_SO, loss_obj, "-lcudart"])
-    if force or _stale(LOSS_AR, [loss_obj]):
+    # the loss drop-in (fused softmax cross-entropy) and the token log-probabilities: their own shared + static library, no dependency on the attention engine
+    loss_objs = []
+    loss_hdrs = [os.path.join(CSRC, "tc_common.cuh"), os.path.join(HERE, "loss", "loss_internal.h"),
+                 os.path.join(HERE, "..", "include", "kernels", "loss.cuh"), os.path.join(HERE, "..", "include", "b200loss.h")]
+    for name in ("cross_entropy", "token_logprobs"):
+        src = os.path.join(HERE, "loss", name + ".cu")
+        obj = os.path.join(OBJDIR, name + ".o")
+        loss_objs.append(obj)
+        if force or _stale(obj, [src] + loss_hdrs):
+            subprocess.check_call([nvcc] + ARCH + FLAGS + (["-Xptxas", "-v"] if ptxas_info else []) +
+                                  ["-I", os.path.join(HERE, "..", "include"), "-I", CSRC, "-c", src, "-o", obj])
+    if force or _stale(LOSS_SO, loss_objs):
+        subprocess.check_call([nvcc] + ARCH + ["-shared", "-o", LOSS_SO] + loss_objs + ["-lcudart"])
+    if force or _stale(LOSS_AR, loss_objs):
         if os.path.exists(LOSS_AR):
             os.remove(LOSS_AR)
-        subprocess.check_call(["ar", "rcs", LOSS_AR, loss_obj])
+        subprocess.check_call(["ar", "rcs", LOSS_AR] + loss_objs)
     # the LayerNorm drop-in (static library only: its interface is the C++ header of the reference)
     norm_src = os.path.join(HERE, "norm", "layernorm_dropin.cu")
     norm_obj = os.path.join(OBJDIR, "layernorm_dropin.o")

@@ -32,6 +32,7 @@
 #include <string>
 
 #include "b200loss.h"
+#include "loss_internal.h"
 #include "tc_common.cuh"
 
 // Defined by the GEMM drop-in (libb200gemm.a) when it is linked into the same program and B200GEMM_TWINS=1, else NULL: a
@@ -327,7 +328,7 @@ __global__ void __launch_bounds__(kStreamThreads)
 }
 
 // ---------------------------------------------------------------- host side
-thread_local std::string g_last_error;
+thread_local char g_last_error[512] = "";
 
 struct DeviceScratch {
     float* row_loss = nullptr;
@@ -341,7 +342,7 @@ DeviceScratch g_scratch[kMaxDevices];
 std::mutex g_mutex;
 
 int fail(int code, const std::string& what) {
-    g_last_error = what;
+    b200loss::set_error(what.c_str());
     return code;
 }
 int cuda_fail(const char* what, cudaError_t e) {
@@ -405,6 +406,11 @@ int launch(const float* logits, const int* targets, float* dlogits, float* devic
 
 }  // namespace
 
+void b200loss::set_error(const char* what, const char* detail) {
+    if (detail) snprintf(g_last_error, sizeof g_last_error, "%s: %s", what, detail);
+    else snprintf(g_last_error, sizeof g_last_error, "%s", what);
+}
+
 extern "C" {
 
 int b200loss_cross_entropy(const float* logits, const int* targets, float* d_logits, float* device_loss, int B, int T,
@@ -442,21 +448,21 @@ void b200loss_release(void) {
     s = DeviceScratch{};
 }
 
-const char* b200loss_last_error(void) { return g_last_error.c_str(); }
+const char* b200loss_last_error(void) { return g_last_error; }
 
 }  // extern "C"
 
 void cross_entropy_forward_backward_device(const float* logits, const int* targets, float* dlogits, float* device_loss, int B,
                                            int T, int V, cudaStream_t stream) {
     if (launch(logits, targets, dlogits, device_loss, device_loss != nullptr, B, T, V, stream, nullptr) != B200LOSS_OK)
-        fprintf(stderr, "[b200loss] %s\n", g_last_error.c_str());
+        fprintf(stderr, "[b200loss] %s\n", g_last_error);
 }
 
 void cross_entropy_forward_backward(const float* logits, const int* targets, float* dlogits, float* host_loss, int B, int T,
                                     int V, cudaStream_t stream) {
     float* where = nullptr;
     if (launch(logits, targets, dlogits, nullptr, host_loss != nullptr, B, T, V, stream, &where) != B200LOSS_OK) {
-        fprintf(stderr, "[b200loss] %s\n", g_last_error.c_str());
+        fprintf(stderr, "[b200loss] %s\n", g_last_error);
         return;
     }
     if (host_loss != nullptr) {

@@ -1,9 +1,12 @@
 """ctypes binding of lib/libb200loss.so (include/b200loss.h) and the launcher of the reference's loss header over it.
 
 `cross_entropy_forward_backward` keeps the name and argument meaning of include/kernels/loss.cuh:8-15 of
-sarimahsan/transformer-cuda with torch CUDA tensors in place of raw pointers. There is no fallback: a missing
-library raises."""
+sarimahsan/transformer-cuda with torch CUDA tensors in place of raw pointers. `token_logprobs_forward` and
+`token_logprobs_backward` (no counterpart there) score given tokens and differentiate that. There is no fallback: a
+missing library raises."""
+import collections
 import ctypes
+import math
 import os
 import re
 
@@ -11,9 +14,11 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 SO_PATH = os.path.join(HERE, "lib", "libb200loss.so")
 HEADER_PATH = os.path.join(HERE, "..", "include", "b200loss.h")
 
-_P, _I = ctypes.c_void_p, ctypes.c_int
+_P, _I, _LL, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_float
 _SIGNATURES = {
     "b200loss_cross_entropy": ([_P, _P, _P, _P, _I, _I, _I, _P], _I),
+    "b200loss_token_logprobs": ([_P, _I, _LL, _P, _I, _I, _F, _P, _P, _P, _I, _P, _P, _P], _I),
+    "b200loss_token_logprobs_backward": ([_P, _I, _LL, _P, _P, _P, _P, _P, _I, _I, _F, _P, _LL, _P], _I),
     "b200loss_kernel_path": ([_P, _P, _I], _I),
     "b200loss_max_resident_vocab": ([], _I),
     "b200loss_check_device_fault": ([], _I),
@@ -72,6 +77,88 @@ def cross_entropy_forward_backward(logits, targets, dlogits=None, want_loss=True
         _check(load().b200loss_cross_entropy(logits.data_ptr(), targets.data_ptr(), dlogits.data_ptr(),
                                              loss.data_ptr() if want_loss else None, B, T, V, stream))
     return dlogits, loss
+
+
+TokenLogprobs = collections.namedtuple("TokenLogprobs", "logprobs entropy stats top_logprobs top_tokens temperature")
+MAX_TOP = 32
+
+
+def _rows(t, name, shape=None):
+    """(rows, V, row stride) of FP32 or BF16 rows (..., V): contiguous elements, one stride from row to row."""
+    import torch
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in (torch.float32, torch.bfloat16) or t.dim() < 1 or t.shape[-1] < 1:
+        raise ValueError(f"{name} must be a CUDA float32 or bfloat16 tensor of shape (..., V)")
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, has {tuple(t.shape)}")
+    V, lead = t.shape[-1], [(n, st) for n, st in zip(t.shape[:-1], t.stride()[:-1]) if n != 1]
+    rows = math.prod(t.shape[:-1])
+    stride = lead[-1][1] if lead else V
+    regular = all(a[1] == b[0] * b[1] for a, b in zip(lead, lead[1:]))
+    if rows and ((t.stride(-1) != 1 and V > 1) or not regular or stride < V):
+        raise ValueError(f"{name} must consist of contiguous rows at one row stride (strides {t.stride()})")
+    return rows, V, stride
+
+
+def _per_row(t, name, dtype, logits, rows):
+    import torch
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != logits.device or not t.is_contiguous() or t.numel() != rows:
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor on the logits' device with one element per row ({rows})")
+    return t.data_ptr()
+
+
+def token_logprobs_forward(logits, targets, temperature=1.0, top=0):
+    """Log-probability of a given token in every row, the row's entropy and its `top` most likely tokens, in one read of
+    the logits. logits (..., V) float32 or bfloat16, rows at one stride (a slice of a wider, padded buffer will do); targets
+    (...) int32, a value outside [0, V) marks padding (log-probability 0). The distribution is softmax(logits / temperature).
+
+    Returns TokenLogprobs: logprobs, entropy (...) and stats (..., 2) float32, top_logprobs (..., top) float32 and top_tokens
+    (..., top) int32 (None when top = 0; larger logits first, equal ones by the lower index; top <= min(32, V)), and the
+    temperature. -inf logits are tokens that are not allowed; see include/b200loss.h for rows without any and for NaN."""
+    import torch
+    rows, V, stride = _rows(logits, "logits")
+    lead = logits.shape[:-1]
+    t_ptr = _per_row(targets, "targets", torch.int32, logits, rows)
+    if not 0 <= int(top) <= min(MAX_TOP, V):
+        raise ValueError(f"top must be between 0 and min({MAX_TOP}, V), got {top}")
+    dev, f32 = logits.device, torch.float32
+    logprobs, entropy = (torch.empty(lead, dtype=f32, device=dev) for _ in range(2))
+    stats = torch.empty(*lead, 2, dtype=f32, device=dev)
+    top_logprobs = torch.empty(*lead, top, dtype=f32, device=dev) if top else None
+    top_tokens = torch.empty(*lead, top, dtype=torch.int32, device=dev) if top else None
+    with torch.cuda.device(dev):
+        _check(load().b200loss_token_logprobs(logits.data_ptr(), int(logits.dtype == torch.bfloat16), stride, t_ptr, rows, V,
+                                              float(temperature), logprobs.data_ptr(), entropy.data_ptr(), stats.data_ptr(),
+                                              int(top), top_logprobs.data_ptr() if top else None,
+                                              top_tokens.data_ptr() if top else None,
+                                              torch.cuda.current_stream(dev).cuda_stream))
+    return TokenLogprobs(logprobs, entropy, stats, top_logprobs, top_tokens, float(temperature))
+
+
+def token_logprobs_backward(logits, targets, result, grad_logprobs, grad_entropy=None, dlogits=None):
+    """Gradient of sum(grad_logprobs * logprobs + grad_entropy * entropy) with regard to the logits that
+    `token_logprobs_forward(logits, targets, ...)` returned `result` for. grad_* (...) float32; dlogits: the logits' shape and
+    type, allocated when not given, may be `logits` itself. Rows that no gradient reaches are zeros."""
+    import torch
+    rows, V, stride = _rows(logits, "logits")
+    t_ptr = _per_row(targets, "targets", torch.int32, logits, rows)
+    f32 = torch.float32
+    e_ptr = _per_row(result.entropy, "result.entropy", f32, logits, rows)
+    s_ptr = _per_row(result.stats, "result.stats", f32, logits, 2 * rows)
+    g_ptr = _per_row(grad_logprobs, "grad_logprobs", f32, logits, rows)
+    ge_ptr = None if grad_entropy is None else _per_row(grad_entropy, "grad_entropy", f32, logits, rows)
+    if dlogits is None:
+        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    elif dlogits.dtype != logits.dtype or dlogits.device != logits.device:
+        raise ValueError("dlogits must have the logits' type and device")
+    _, _, d_stride = _rows(dlogits, "dlogits", logits.shape)
+    if dlogits.data_ptr() == logits.data_ptr() and d_stride != stride:
+        raise ValueError("dlogits in the logits' place must have the logits' row stride")
+    with torch.cuda.device(logits.device):
+        _check(load().b200loss_token_logprobs_backward(logits.data_ptr(), int(logits.dtype == torch.bfloat16), stride, t_ptr,
+                                                       e_ptr, s_ptr, g_ptr, ge_ptr, rows, V, result.temperature,
+                                                       dlogits.data_ptr(), d_stride,
+                                                       torch.cuda.current_stream(logits.device).cuda_stream))
+    return dlogits
 
 
 def kernel_path(logits, dlogits):
