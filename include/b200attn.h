@@ -176,6 +176,39 @@ int b200attn_bwd_bf16_packed(const void* qkv, const void* out, const void* dout,
 int b200attn_bwd_bf16_noalloc(const void* q, const void* k, const void* v, const void* o, const void* dO,
                               const float* lse, void* dq, void* dk, void* dv, int BH, int T, int d, float scale,
                               b200attn_stream_t stream);
+/* Causal attention over packed sequences of different lengths with grouped heads. q (total, H, d), k and v (total, Hkv, d)
+ * BF16, H a multiple of Hkv: query head h reads key head h / (H / Hkv). Sequence i is rows offsets[i] .. offsets[i + 1] - 1
+ * (`offsets`: n + 1 ascending ints on the DEVICE, clipped to [0, total]; a sequence may be empty); a query sees the keys
+ * of its own sequence up to itself. out (total, H, d) BF16, lse (H, total) FP32. Heads are contiguous (stride d), rows are
+ * *_stride elements apart (a multiple of 8), so q, k and v may be parts of one projection output. Rows that belong to no sequence
+ * are not read into any result and keep their values in out and lse. d in {64, 128}, scale > 0; 16-byte aligned tensors.
+ * `workspace` (caller-owned, b200attn_ragged_workspace_bytes(total, n, H, d, 0) bytes, 16-byte aligned) is written by the
+ * call; calls that may run at the same time need workspaces of their own. No counterpart in the reference. */
+long long b200attn_ragged_workspace_bytes(int total, int n, int H, int d, int backward);
+int b200attn_fwd_bf16_ragged(const void* q, const void* k, const void* v, const int* offsets, void* out, float* lse,
+                             void* workspace, long long workspace_bytes, int total, int n, int H, int Hkv, int d,
+                             long long q_stride, long long kv_stride, long long out_stride, float scale,
+                             b200attn_stream_t stream);
+/* Its backward: dq (total, H, d), dk and dv (total, Hkv, d) BF16 of the rows that belong to a sequence, overwritten (dk and
+ * dv summed over the query heads of a group), from the forward's out and lse and from dout (total, H, d). Workspace:
+ * b200attn_ragged_workspace_bytes(total, n, H, d, 1) bytes. dQ is summed in FP32 in an order that is not fixed, like that of
+ * b200attn_bwd_bf16. */
+int b200attn_bwd_bf16_ragged(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse,
+                             const int* offsets, void* dq, void* dk, void* dv, void* workspace, long long workspace_bytes,
+                             int total, int n, int H, int Hkv, int d, long long q_stride, long long kv_stride,
+                             long long out_stride, long long dout_stride, long long dq_stride, long long dkv_stride, float scale,
+                             b200attn_stream_t stream);
+/* The same for ONE new query token of each of B sequences over a cache: q (B, H, d) at q_stride elements, keys and values
+ * BF16 at cache + b * batch_stride + t * row_stride + h * head_stride (+ e), t < T, all strides multiples of 8 elements, so
+ * (B, T, Hkv, d) and (B, Hkv, T, d) caches both fit. lengths[b] (device, clipped to [0, T]): the keys the token sees, its
+ * own included once it is in the cache; rows behind them are not read. out (B, H, d) BF16, lse (B, H) FP32, both dense; a
+ * sequence of length 0 gets zeros and -inf. Workspace: b200attn_decode_workspace_bytes bytes (0: may be NULL). The result
+ * does not depend on timing. No counterpart in the reference. */
+long long b200attn_decode_workspace_bytes(int B, int T, int H, int Hkv, int d);
+int b200attn_decode_bf16(const void* q, const void* k_cache, const void* v_cache, const int* lengths, void* out, float* lse,
+                         void* workspace, long long workspace_bytes, int B, int T, int H, int Hkv, int d, long long q_stride,
+                         long long k_batch_stride, long long k_row_stride, long long k_head_stride, long long v_batch_stride,
+                         long long v_row_stride, long long v_head_stride, float scale, b200attn_stream_t stream);
 /* FP32 (B,T,3*H*d) -> BF16 q,k,v (B,H,T,d): the split-transpose fused with the down-conversion
  * (same index map as src/kernels/attention.cu:24-83). */
 int b200attn_qkv_split_bf16(const float* qkv, void* q, void* k, void* v, int B, int T, int H, int d,

@@ -815,6 +815,215 @@ extern "C" int b200attn_bwd_bf16_packed(const void* qkv, const void* out, const 
     return B200ATTN_OK;
 }
 
+// ---------------------------------------------------------------------- packed sequences of different lengths
+namespace {
+
+// What the calls below carve out of the caller's workspace.
+struct RaggedSpace {
+    int capacity;  // work items at most
+    int4* items;
+    int* count;              // [0] number of items, [1] work counter of the persistent backward
+    float *dq_acc, *D, *lse2;
+    __nv_bfloat16 *lse_ext, *d_ext;
+    size_t bytes;
+};
+RaggedSpace ragged_space(void* base, int total, int n, int H, int d, bool backward) {
+    RaggedSpace s{};
+    const long long tiles = (long long)total / 128 + n;  // every sequence adds at most one tile that is not full
+    s.capacity = int(tiles < total ? tiles : total);
+    Bump bump{static_cast<uint8_t*>(base)};
+    s.items = bump.take<int4>(size_t(s.capacity));
+    s.count = bump.take<int>(2);
+    if (backward) {
+        const size_t rows = size_t(total) * H;
+        s.dq_acc = bump.take<float>(rows * d);
+        s.D = bump.take<float>(rows);
+        s.lse2 = bump.take<float>(rows);
+        if (d == 64) {
+            s.lse_ext = bump.take<__nv_bfloat16>(rows * 16);
+            s.d_ext = bump.take<__nv_bfloat16>(rows * 16);
+        }
+    }
+    s.bytes = size_t(bump.p - static_cast<uint8_t*>(base));
+    return s;
+}
+
+bool row_stride_ok(long long stride, long long width) { return stride >= width && stride % 8 == 0 && stride < (1LL << 36); }
+
+int check_ragged(const char* fn, int total, int n, int H, int Hkv, int d, float scale) {
+    if (total < 0 || n < 0 || H <= 0 || Hkv <= 0) return fail(B200ATTN_ERR_INVALID_ARGUMENT, "%s: negative size or no heads (total=%d n=%d H=%d Hkv=%d)", fn, total, n, H, Hkv);
+    if (H % Hkv != 0) return fail(B200ATTN_ERR_INVALID_ARGUMENT, "%s: H=%d is not a multiple of Hkv=%d", fn, H, Hkv);
+    if (total > (1 << 30) || n > (1 << 30) || H > 65535) return fail(B200ATTN_ERR_UNSUPPORTED, "%s: more than 2^30 rows or sequences or 65535 heads", fn);
+    if (d != 64 && d != 128) return fail(B200ATTN_ERR_UNSUPPORTED, "%s: supports d in {64,128}, got %d", fn, d);
+    if (!(scale > 1e-20f && scale < 1e20f)) return fail(B200ATTN_ERR_INVALID_ARGUMENT, "%s: scale must be positive and between 1e-20 and 1e20", fn);
+    return B200ATTN_OK;
+}
+// (d, total, heads, 1) view of packed rows at `stride` elements
+Layout ragged_layout(long long stride, int d) { return Layout{stride, d, stride}; }
+
+}  // namespace
+
+extern "C" long long b200attn_ragged_workspace_bytes(int total, int n, int H, int d, int backward) {
+    if (total < 0 || n < 0 || H <= 0 || d <= 0) return 0;
+    return (long long)ragged_space(nullptr, total, n, H, d, backward != 0).bytes;
+}
+
+extern "C" int b200attn_fwd_bf16_ragged(const void* q, const void* k, const void* v, const int* offsets, void* out, float* lse,
+                                        void* workspace, long long workspace_bytes, int total, int n, int H, int Hkv, int d,
+                                        long long q_stride, long long kv_stride, long long out_stride, float scale,
+                                        b200attn_stream_t stream_) {
+    const char* fn = "b200attn_fwd_bf16_ragged";
+    cudaStream_t stream = (cudaStream_t)stream_;
+    int rc = check_ragged(fn, total, n, H, Hkv, d, scale);
+    if (rc) return rc;
+    if (total == 0 || n == 0) return B200ATTN_OK;
+    REQUIRE_PTR(fn, q); REQUIRE_PTR(fn, k); REQUIRE_PTR(fn, v); REQUIRE_PTR(fn, offsets); REQUIRE_PTR(fn, out); REQUIRE_PTR(fn, lse);
+    REQUIRE_PTR(fn, workspace);
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(workspace))
+        return fail(B200ATTN_ERR_INVALID_ARGUMENT, "%s: tensors and workspace must be 16-byte aligned", fn);
+    if (!row_stride_ok(q_stride, (long long)H * d) || !row_stride_ok(kv_stride, (long long)Hkv * d) || !row_stride_ok(out_stride, (long long)H * d))
+        return fail(B200ATTN_ERR_INVALID_ARGUMENT, "%s: a row stride is smaller than its heads, not a multiple of 8 elements or too large", fn);
+    const RaggedSpace s = ragged_space(workspace, total, n, H, d, false);
+    if (workspace_bytes < (long long)s.bytes)
+        return fail(B200ATTN_ERR_SCRATCH, "%s: workspace of %lld bytes, needs %zu (b200attn_ragged_workspace_bytes)", fn, workspace_bytes, s.bytes);
+    if ((long long)s.capacity * H > 0x7fffffffLL) return fail(B200ATTN_ERR_UNSUPPORTED, "%s: too many tiles", fn);
+    DeviceState* st = nullptr;
+    if ((rc = device_state(stream, &st))) return rc;
+    if ((rc = tc_supported(fn, st, d))) return rc;
+    TcFwdArgs a;
+    memset(&a, 0, sizeof(a));
+    if ((rc = make_map(&a.map_q, q, false, 1, H, total, d, ragged_layout(q_stride, d)))) return rc;
+    if ((rc = make_map(&a.map_k, k, false, 1, Hkv, total, d, ragged_layout(kv_stride, d)))) return rc;
+    if ((rc = make_map(&a.map_v, v, false, 1, Hkv, total, d, ragged_layout(kv_stride, d)))) return rc;
+    if ((rc = make_map(&a.map_o, out, false, 1, H, total, d, ragged_layout(out_stride, d)))) return rc;
+    a.out = out;
+    a.lse_out = lse;
+    a.BH = H, a.T = total, a.d = d, a.H = H;
+    a.scale = scale;
+    a.fault_word = st->fault_word;
+    a.ragged = RaggedWork{s.items, s.count, s.capacity, H / Hkv, Hkv, out_stride};
+    RETURN_IF_CUDA(launch_ragged_plan(offsets, n, total, s.items, s.count, s.capacity, nullptr, stream), "work list launch");
+    ScopedKernelTimer timer(0, stream);
+    RETURN_IF_CUDA(launch_attn_fwd_ragged(a, stream), "packed forward launch");
+    return B200ATTN_OK;
+}
+
+extern "C" int b200attn_bwd_bf16_ragged(const void* q, const void* k, const void* v, const void* out, const void* dout,
+                                        const float* lse, const int* offsets, void* dq, void* dk, void* dv, void* workspace,
+                                        long long workspace_bytes, int total, int n, int H, int Hkv, int d, long long q_stride,
+                                        long long kv_stride, long long out_stride, long long dout_stride, long long dq_stride,
+                                        long long dkv_stride, float scale, b200attn_stream_t stream_) {
+    const char* fn = "b200attn_bwd_bf16_ragged";
+    cudaStream_t stream = (cudaStream_t)stream_;
+    int rc = check_ragged(fn, total, n, H, Hkv, d, scale);
+    if (rc) return rc;
+    if (total == 0 || n == 0) return B200ATTN_OK;
+    REQUIRE_PTR(fn, q); REQUIRE_PTR(fn, k); REQUIRE_PTR(fn, v); REQUIRE_PTR(fn, out); REQUIRE_PTR(fn, dout); REQUIRE_PTR(fn, lse);
+    REQUIRE_PTR(fn, offsets); REQUIRE_PTR(fn, dq); REQUIRE_PTR(fn, dk); REQUIRE_PTR(fn, dv); REQUIRE_PTR(fn, workspace);
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) || !aligned16(dout) || !aligned16(dq) || !aligned16(dk) ||
+        !aligned16(dv) || !aligned16(workspace))
+        return fail(B200ATTN_ERR_INVALID_ARGUMENT, "%s: tensors and workspace must be 16-byte aligned", fn);
+    const long long wq = (long long)H * d, wk = (long long)Hkv * d;
+    if (!row_stride_ok(q_stride, wq) || !row_stride_ok(kv_stride, wk) || !row_stride_ok(out_stride, wq) || !row_stride_ok(dout_stride, wq) ||
+        !row_stride_ok(dq_stride, wq) || !row_stride_ok(dkv_stride, wk))
+        return fail(B200ATTN_ERR_INVALID_ARGUMENT, "%s: a row stride is smaller than its heads, not a multiple of 8 elements or too large", fn);
+    const RaggedSpace s = ragged_space(workspace, total, n, H, d, true);
+    if (workspace_bytes < (long long)s.bytes)
+        return fail(B200ATTN_ERR_SCRATCH, "%s: workspace of %lld bytes, needs %zu (b200attn_ragged_workspace_bytes)", fn, workspace_bytes, s.bytes);
+    if ((long long)s.capacity * Hkv > 0x7fffffffLL || (long long)total * H * (d / 8) / 256 > 0x7ffffff0LL)
+        return fail(B200ATTN_ERR_UNSUPPORTED, "%s: too many tiles", fn);
+    DeviceState* st = nullptr;
+    if ((rc = device_state(stream, &st))) return rc;
+    if ((rc = tc_supported(fn, st, d))) return rc;
+    TcBwdArgs a;
+    memset(&a, 0, sizeof(a));
+    if ((rc = make_map(&a.map_q, q, false, 1, H, total, d, ragged_layout(q_stride, d)))) return rc;
+    if ((rc = make_map(&a.map_k, k, false, 1, Hkv, total, d, ragged_layout(kv_stride, d)))) return rc;
+    if ((rc = make_map(&a.map_v, v, false, 1, Hkv, total, d, ragged_layout(kv_stride, d)))) return rc;
+    if ((rc = make_map(&a.map_do, dout, false, 1, H, total, d, ragged_layout(dout_stride, d)))) return rc;
+    if ((rc = make_map(&a.map_dk, dk, false, 1, Hkv, total, d, ragged_layout(dkv_stride, d)))) return rc;
+    if ((rc = make_map(&a.map_dv, dv, false, 1, Hkv, total, d, ragged_layout(dkv_stride, d)))) return rc;
+    if ((rc = make_map(&a.map_dq_acc, s.dq_acc, true, 1, H, total, d, ragged_layout(wq, d)))) return rc;
+    a.lse2 = s.lse2, a.D = s.D, a.dq_acc = s.dq_acc;
+    a.dk = dk, a.dv = dv;
+    a.BH = H, a.T = total, a.d = d, a.H = H;
+    a.scale = scale;
+    a.fault_word = st->fault_word;
+    a.grad_lt = dkv_stride, a.grad_lh = d, a.grad_lb = 0;
+    a.ragged = RaggedWork{s.items, s.count, s.capacity, H / Hkv, Hkv, dkv_stride};
+    BwdStatRows ext{nullptr, nullptr, 0.f};
+    if (d == 64) {
+        ext = BwdStatRows{s.lse_ext, s.d_ext, 1.0f / scale};
+        if ((rc = make_stat_map(&a.map_lse_ext, s.lse_ext, 1, H, total))) return rc;
+        if ((rc = make_stat_map(&a.map_d_ext, s.d_ext, 1, H, total))) return rc;
+        a.work_counter = reinterpret_cast<unsigned int*>(s.count + 1);
+    }
+    RETURN_IF_CUDA(launch_ragged_plan(offsets, n, total, s.items, s.count, s.capacity, a.work_counter, stream), "work list launch");
+    RETURN_IF_CUDA(launch_ragged_prepass(static_cast<const __nv_bfloat16*>(out), out_stride, static_cast<const __nv_bfloat16*>(dout),
+                                         dout_stride, lse, s.D, s.lse2, s.dq_acc, total, H, d, ext, stream), "pre-pass");
+    {
+        ScopedKernelTimer timer(1, stream);
+        RETURN_IF_CUDA(d == 64 ? launch_attn_bwd_ragged64(a, stream) : launch_attn_bwd_ragged128(a, stream), "packed backward launch");
+    }
+    // the head-dim-64 kernel leaves the softmax scale out of dS: dK is scaled where it is stored, dQ here
+    RETURN_IF_CUDA(launch_ragged_dq_convert(s.dq_acc, static_cast<__nv_bfloat16*>(dq), dq_stride, offsets, n, total, H, d,
+                                            d == 64 ? scale : 1.0f, stream), "dq convert");
+    return B200ATTN_OK;
+}
+
+// ---------------------------------------------------------------------- one new token per sequence
+extern "C" long long b200attn_decode_workspace_bytes(int B, int T, int H, int Hkv, int d) {
+    if (B <= 0 || T <= 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || d <= 0) return 0;
+    const int splits = decode_splits(B, T, H, Hkv);
+    return splits == 1 ? 0 : (long long)B * H * splits * (d + 2) * (long long)sizeof(float);
+}
+
+extern "C" int b200attn_decode_bf16(const void* q, const void* k_cache, const void* v_cache, const int* lengths, void* out, float* lse,
+                                    void* workspace, long long workspace_bytes, int B, int T, int H, int Hkv, int d, long long q_stride,
+                                    long long k_batch_stride, long long k_row_stride, long long k_head_stride, long long v_batch_stride,
+                                    long long v_row_stride, long long v_head_stride, float scale, b200attn_stream_t stream_) {
+    const char* fn = "b200attn_decode_bf16";
+    cudaStream_t stream = (cudaStream_t)stream_;
+    if (B < 0 || T < 0 || H <= 0 || Hkv <= 0) return fail(B200ATTN_ERR_INVALID_ARGUMENT, "%s: negative size or no heads (B=%d T=%d H=%d Hkv=%d)", fn, B, T, H, Hkv);
+    if (H % Hkv != 0) return fail(B200ATTN_ERR_INVALID_ARGUMENT, "%s: H=%d is not a multiple of Hkv=%d", fn, H, Hkv);
+    if (d != 64 && d != 128) return fail(B200ATTN_ERR_UNSUPPORTED, "%s: supports d in {64,128}, got %d", fn, d);
+    if (B > 65535 || H > 32768) return fail(B200ATTN_ERR_UNSUPPORTED, "%s: more than 65535 sequences or 32768 heads", fn);
+    if (T > (1 << 30)) return fail(B200ATTN_ERR_UNSUPPORTED, "%s: capacity above 2^30", fn);
+    if (!(scale > 0.f) || !(scale < 1e20f)) return fail(B200ATTN_ERR_INVALID_ARGUMENT, "%s: scale must be positive and finite", fn);
+    if (B == 0) return B200ATTN_OK;
+    REQUIRE_PTR(fn, q); REQUIRE_PTR(fn, lengths); REQUIRE_PTR(fn, out); REQUIRE_PTR(fn, lse);
+    if (T > 0) { REQUIRE_PTR(fn, k_cache); REQUIRE_PTR(fn, v_cache); }
+    if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(out) || !aligned16(workspace))
+        return fail(B200ATTN_ERR_INVALID_ARGUMENT, "%s: tensors and workspace must be 16-byte aligned", fn);
+    const long long strides[7] = {q_stride, k_batch_stride, k_row_stride, k_head_stride, v_batch_stride, v_row_stride, v_head_stride};
+    for (long long x : strides)
+        if (x < 0 || x % 8 != 0) return fail(B200ATTN_ERR_INVALID_ARGUMENT, "%s: strides must be multiples of 8 elements and not negative", fn);
+    const long long need = b200attn_decode_workspace_bytes(B, T, H, Hkv, d);
+    if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+        return fail(B200ATTN_ERR_SCRATCH, "%s: workspace of %lld bytes, needs %lld (b200attn_decode_workspace_bytes)", fn, workspace ? workspace_bytes : 0LL, need);
+    DeviceState* st = nullptr;
+    int rc;
+    if ((rc = device_state(stream, &st))) return rc;
+    if ((rc = tc_supported(fn, st, d))) return rc;
+    DecodeArgs a;
+    memset(&a, 0, sizeof(a));
+    a.q = static_cast<const __nv_bfloat16*>(q), a.k = static_cast<const __nv_bfloat16*>(k_cache), a.v = static_cast<const __nv_bfloat16*>(v_cache);
+    a.lengths = lengths;
+    a.out = static_cast<__nv_bfloat16*>(out), a.lse = lse;
+    a.B = B, a.T = T, a.H = H, a.Hkv = Hkv, a.d = d;
+    a.q_stride = q_stride;
+    a.k_batch = k_batch_stride, a.k_row = k_row_stride, a.k_head = k_head_stride;
+    a.v_batch = v_batch_stride, a.v_row = v_row_stride, a.v_head = v_head_stride;
+    a.scale = scale;
+    a.splits = T > 0 ? decode_splits(B, T, H, Hkv) : 1;
+    if (a.splits > 1) {
+        a.part_o = static_cast<float*>(workspace);
+        a.part_ml = a.part_o + (long long)B * H * a.splits * d;
+    }
+    RETURN_IF_CUDA(launch_attn_decode(a, stream), "single-token attention launch");
+    return B200ATTN_OK;
+}
+
 extern "C" int b200attn_qkv_split_bf16(const float* qkv, void* q, void* k, void* v, int B, int T, int H, int d,
                                        b200attn_stream_t stream) {
     const char* fn = "b200attn_qkv_split_bf16";

@@ -1,0 +1,192 @@
+// The passes around the attention kernels for packed sequences of different lengths: the list of work items, the backward's
+// pre-pass over O and dO, and the conversion of the dQ sums. (The attention itself: the RAGGED instances of
+// attn_tc_fwd_short.cu, attn_tc_bwd.cu and attn_tc_bwd64.cu.)
+#include "kernels.cuh"
+#include "tc_common.cuh"
+
+namespace b200attn {
+namespace {
+
+constexpr int kTile = 128;
+constexpr float kLog2e = 1.4426950408889634f;
+
+// ------------------------------------------------------------------ work items
+// One CTA. A sequence of n tiles gives n items that walk 1 .. n tiles; they are listed by descending number, so that the long
+// ones start first and the tail of the launch is short: a counting sort over the numbers (grouped by `shift` where a sequence
+// can have more than kLevels tiles). The order inside a level is that of arrival; no result depends on it.
+constexpr int kPlanThreads = 1024;
+constexpr int kLevels = 4096;
+
+__device__ __forceinline__ int2 sequence_rows(const int* offsets, int i, int T) {  // first row and length, within [0, T]
+    const int a = min(max(offsets[i], 0), T), b = min(max(offsets[i + 1], a), T);
+    return make_int2(a, b - a);
+}
+
+__global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(const int* __restrict__ offsets, int n, int T, int4* __restrict__ items,
+                                                                   int* __restrict__ count, int capacity, unsigned int* counter, int shift) {
+    __shared__ int level[kLevels];
+    __shared__ int warp_total[32];
+    __shared__ int s_levels;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    pdl_launch_dependents();
+    pdl_wait();
+    // Calls visit(first row, length, tiles) for every item of the sequences i = tid, tid + 1024, ...: short sequences by the
+    // thread that holds them, long ones by its whole warp.
+    auto for_items = [&](auto&& visit) {
+        for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
+            const int i = i0 + tid;
+            const int2 s = i < n ? sequence_rows(offsets, i, T) : make_int2(0, 0);
+            const int tiles = (s.y + kTile - 1) / kTile;
+            if (tiles <= 8)
+                for (int c = 1; c <= tiles; ++c) visit(s.x, s.y, c);
+            uint32_t more = __ballot_sync(0xffffffffu, tiles > 8);
+            while (more) {
+                const int src = __ffs(more) - 1;
+                more &= more - 1;
+                const int x = __shfl_sync(0xffffffffu, s.x, src), y = __shfl_sync(0xffffffffu, s.y, src);
+                for (int c = 1 + lane; c <= (y + kTile - 1) / kTile; c += 32) visit(x, y, c);
+            }
+        }
+    };
+    const int levels = min(kLevels, (((T + kTile - 1) / kTile - 1) >> shift) + 1);
+    for (int i = tid; i < levels; i += kPlanThreads) level[i] = 0;
+    __syncthreads();
+    // level l (descending): position 0 is the longest
+    for_items([&](int, int, int c) { atomicAdd(&level[levels - 1 - ((c - 1) >> shift)], 1); });
+    __syncthreads();
+    // exclusive prefix sum over the levels, kLevels / 1024 neighbours per thread
+    constexpr int kPer = kLevels / kPlanThreads;
+    int v[kPer], sum = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int at = tid * kPer + i;
+        v[i] = at < levels ? level[at] : 0;
+        sum += v[i];
+    }
+    int incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+    }
+    if (lane == 31) warp_total[warp] = incl;
+    __syncthreads();
+    if (warp == 0) {
+        int x = warp_total[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        warp_total[lane] = x;
+        if (lane == 31) s_levels = x;
+    }
+    __syncthreads();
+    int at_item = incl - sum + (warp ? warp_total[warp - 1] : 0);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+        const int at = tid * kPer + i;
+        if (at < levels) level[at] = at_item;
+        at_item += v[i];
+    }
+    __syncthreads();
+    // offsets that are not in ascending order could make more items than fit: those behind the list are dropped
+    for_items([&](int row, int len, int c) {
+        const int at = atomicAdd(&level[levels - 1 - ((c - 1) >> shift)], 1);
+        if (at < capacity) items[at] = make_int4(row, len, c, 0);
+    });
+    if (tid == 0) {
+        *count = min(s_levels, capacity);
+        if (counter) *counter = 0u;
+    }
+}
+
+// ------------------------------------------------------------------ pre-pass
+// Rows in token order (t, h): d / 8 threads per row, 16 bytes each. Writes D = rowsum(dO * O) and the statistics the backward
+// kernels read, (H, T), and clears the dQ sums, (T, H, d).
+__global__ void __launch_bounds__(256) ragged_prepass_kernel(const __nv_bfloat16* __restrict__ o, long long o_stride,
+                                                             const __nv_bfloat16* __restrict__ dO, long long do_stride,
+                                                             const float* __restrict__ lse, float* __restrict__ Dout,
+                                                             float* __restrict__ lse2, float* __restrict__ dq_acc, int T, int H, int d,
+                                                             BwdStatRows ext) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int tpr = d / 8;
+    const long long gid = blockIdx.x * 256ll + threadIdx.x;
+    const long long row = gid / tpr;  // t * H + h
+    const int e = int(gid % tpr) * 8;
+    const bool live = row < (long long)T * H;
+    const int t = int(row / H), h = int(row % H);
+    float acc = 0.f;
+    if (live) {
+        const uint4 ua = __ldg(reinterpret_cast<const uint4*>(o + t * o_stride + (long long)h * d + e));
+        const uint4 ub = __ldg(reinterpret_cast<const uint4*>(dO + t * do_stride + (long long)h * d + e));
+        const __nv_bfloat16* pa = reinterpret_cast<const __nv_bfloat16*>(&ua);
+        const __nv_bfloat16* pb = reinterpret_cast<const __nv_bfloat16*>(&ub);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) acc = fmaf(__bfloat162float(pa[x]), __bfloat162float(pb[x]), acc);
+        float4* z = reinterpret_cast<float4*>(dq_acc + row * d + e);
+        z[0] = make_float4(0.f, 0.f, 0.f, 0.f);
+        z[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    for (int off = tpr >> 1; off > 0; off >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, off);
+    if (live && e == 0) {
+        const long long at = (long long)h * T + t;
+        const float x = lse[at];
+        Dout[at] = acc;
+        lse2[at] = x * kLog2e;
+        if (ext.lse_ext) {
+            store_stat_row(ext.lse_ext + at * 16, x * ext.inv_scale);
+            store_stat_row(ext.d_ext + at * 16, acc);
+        }
+    }
+}
+
+__global__ void __launch_bounds__(256) ragged_dq_convert_kernel(const float* __restrict__ acc, __nv_bfloat16* __restrict__ dq,
+                                                                long long dq_stride, const int* __restrict__ offsets, int n, int T, int H,
+                                                                int d, float scale) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int tpr = d / 8;
+    const long long gid = blockIdx.x * 256ll + threadIdx.x;
+    const long long row = gid / tpr;
+    const int e = int(gid % tpr) * 8;
+    const int t = int(row / H), h = int(row % H);
+    if (row >= (long long)T * H || t < offsets[0] || t >= offsets[n]) return;  // rows of no sequence stay as they are
+    const float4 a0 = __ldg(reinterpret_cast<const float4*>(acc + row * d + e));
+    const float4 a1 = __ldg(reinterpret_cast<const float4*>(acc + row * d + e + 4));
+    uint4 w;
+    w.x = pack_bf16x2(a0.x * scale, a0.y * scale);
+    w.y = pack_bf16x2(a0.z * scale, a0.w * scale);
+    w.z = pack_bf16x2(a1.x * scale, a1.y * scale);
+    w.w = pack_bf16x2(a1.z * scale, a1.w * scale);
+    *reinterpret_cast<uint4*>(dq + t * dq_stride + (long long)h * d + e) = w;
+}
+
+}  // namespace
+
+cudaError_t launch_ragged_plan(const int* offsets, int n, int T, int4* items, int* count, int capacity, unsigned int* counter,
+                               cudaStream_t stream) {
+    int shift = 0;
+    while ((((T + kTile - 1) / kTile - 1) >> shift) >= kLevels) ++shift;
+    return launch_pdl(ragged_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, offsets, n, T, items, count, capacity, counter, shift);
+}
+
+cudaError_t launch_ragged_prepass(const __nv_bfloat16* o, long long o_stride, const __nv_bfloat16* dO, long long do_stride,
+                                  const float* lse, float* D, float* lse2, float* dq_acc, int T, int H, int d, BwdStatRows ext,
+                                  cudaStream_t stream) {
+    const long long blocks = ((long long)T * H * (d / 8) + 255) / 256;
+    if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+    return launch_pdl(ragged_prepass_kernel, dim3((unsigned int)blocks), dim3(256), 0, stream, o, o_stride, dO, do_stride, lse, D, lse2,
+                      dq_acc, T, H, d, ext);
+}
+
+cudaError_t launch_ragged_dq_convert(const float* dq_acc, __nv_bfloat16* dq, long long dq_stride, const int* offsets, int n, int T,
+                                     int H, int d, float scale, cudaStream_t stream) {
+    const long long blocks = ((long long)T * H * (d / 8) + 255) / 256;
+    if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+    return launch_pdl(ragged_dq_convert_kernel, dim3((unsigned int)blocks), dim3(256), 0, stream, dq_acc, dq, dq_stride, offsets, n, T, H,
+                      d, scale);
+}
+
+}  // namespace b200attn

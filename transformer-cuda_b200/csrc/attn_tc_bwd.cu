@@ -68,7 +68,9 @@ struct BwdBarriers {
     uint64_t s_full, dp_full, p_ready, ds_ready, dq_full, dq_empty;
 };
 
-template <int D, bool GRADS_F32>
+// RAGGED: packed sequences with grouped heads; a CTA walks the query tiles of all heads of its key head's group, head by head, so
+// that dK and dV of the group are summed in TMEM.
+template <int D, bool GRADS_F32, bool RAGGED>
 __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc_kernel(const __grid_constant__ TcBwdArgs a) {
     using Cfg = BwdCfg<D>;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -94,10 +96,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc_kernel(const __grid_c
     // CTA order. Key tile 0 sees every query tile and is the longest. When the whole problem fits in
     // L2 the CTAs are issued longest-first across ALL slabs (shortest tail); otherwise slab by slab,
     // so that the CTAs resident at one time share few slabs and their tiles stay in L2.
-    const int bh = a.tile_major_order ? int(blockIdx.x % a.BH) : int(blockIdx.x / n_tiles);
-    const int jt = a.tile_major_order ? int(blockIdx.x / a.BH) : int(blockIdx.x % n_tiles);
-    const int hh = bh % a.H, bb = bh / a.H;  // head and batch coordinates of the 4-D tensor maps
-    const int n_it = n_tiles - jt;        // query tiles jt .. n_tiles-1
+    int bh = 0, jt = 0, hh = 0, bb = 0;  // hh, bb: (key) head and batch coordinates of the 4-D tensor maps
+    int n_it = 0;                        // steps: query tiles jt .. n_tiles-1 (RAGGED: of every head of the group)
+    int row0 = 0, len = a.T, n_q = 0;    // RAGGED: the sequence's first row and length; query tiles per head
+    if constexpr (!RAGGED) {
+        bh = a.tile_major_order ? int(blockIdx.x % a.BH) : int(blockIdx.x / n_tiles);
+        jt = a.tile_major_order ? int(blockIdx.x / a.BH) : int(blockIdx.x % n_tiles);
+        hh = bh % a.H, bb = bh / a.H;
+        n_it = n_q = n_tiles - jt;
+    }
 
     if (tid == 0) {
         mbar_init(&bars.k_full, 1);
@@ -129,6 +136,22 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc_kernel(const __grid_c
     // barriers, TMEM and the tensor maps are set up: from here on global memory is touched, so wait for the
     // kernel in front of this one in the stream (returns at once for an ordinary launch)
     pdl_wait();
+    if constexpr (RAGGED) {
+        const int item = int(blockIdx.x / unsigned(a.ragged.kv_heads));
+        if (item >= *a.ragged.count) {
+            __syncthreads();
+            if (warp == kProducerWarp) tmem_dealloc(tmem, Cfg::kTmemCols);
+            return;
+        }
+        const int4 w = a.ragged.items[item];
+        hh = int(blockIdx.x % unsigned(a.ragged.kv_heads));
+        row0 = w.x, len = w.y, n_q = w.z, jt = (len + kBKV - 1) / kBKV - n_q, n_it = n_q * a.ragged.group;
+    }
+    const int valid_kv = RAGGED ? min(kBKV, len - jt * kBKV) : kBKV;  // keys of this tile that belong to the sequence
+    // query tile and head of step `it`, and the tile's rows that belong to the sequence
+    auto q_tile = [&](int it) { return RAGGED ? jt + it % n_q : jt + it; };
+    auto q_head = [&](int it) { return RAGGED ? hh * a.ragged.group + it / n_q : hh; };
+    auto q_valid = [&](int it) { return min(kBQ, len - q_tile(it) * kBQ); };
 
     if (warp == kProducerWarp) {
         // ------------------------------------------------------------ TMA producer
@@ -139,24 +162,24 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc_kernel(const __grid_c
             tma_prefetch_desc(&a.map_do);
             mbar_expect_tx(&bars.k_full, Cfg::kTileBytes);
             for (int at = 0; at < Cfg::kAtoms; ++at)
-                tma_load_4d(sK + at * kAtomBytes, &a.map_k, &bars.k_full, at * 64, jt * kBKV, hh, bb);
+                tma_load_4d(sK + at * kAtomBytes, &a.map_k, &bars.k_full, at * 64, row0 + jt * kBKV, hh, bb);
             mbar_expect_tx(&bars.v_full, Cfg::kTileBytes);
             for (int at = 0; at < Cfg::kAtoms; ++at)
-                tma_load_4d(sV + at * kAtomBytes, &a.map_v, &bars.v_full, at * 64, jt * kBKV, hh, bb);
+                tma_load_4d(sV + at * kAtomBytes, &a.map_v, &bars.v_full, at * 64, row0 + jt * kBKV, hh, bb);
             for (int it = 0; it < n_it; ++it) {
-                const int i = jt + it;
+                const int q_row = row0 + q_tile(it) * kBQ, qh = q_head(it);
                 const int qs = it % Cfg::kQStages;
                 if (it >= Cfg::kQStages)
                     mbar_wait(&bars.q_empty[qs], (it / Cfg::kQStages - 1) & 1, &abort_flag, a.fault_word, 0x40);
                 mbar_expect_tx(&bars.q_full[qs], Cfg::kTileBytes);
                 for (int at = 0; at < Cfg::kAtoms; ++at)
-                    tma_load_4d(sQ + qs * Cfg::kTileBytes + at * kAtomBytes, &a.map_q, &bars.q_full[qs], at * 64, i * kBQ, hh, bb);
+                    tma_load_4d(sQ + qs * Cfg::kTileBytes + at * kAtomBytes, &a.map_q, &bars.q_full[qs], at * 64, q_row, qh, bb);
                 const int os = it % Cfg::kDoStages;
                 if (it >= Cfg::kDoStages)
                     mbar_wait(&bars.do_empty[os], (it / Cfg::kDoStages - 1) & 1, &abort_flag, a.fault_word, 0x41);
                 mbar_expect_tx(&bars.do_full[os], Cfg::kTileBytes);
                 for (int at = 0; at < Cfg::kAtoms; ++at)
-                    tma_load_4d(sDO + os * Cfg::kTileBytes + at * kAtomBytes, &a.map_do, &bars.do_full[os], at * 64, i * kBQ, hh, bb);
+                    tma_load_4d(sDO + os * Cfg::kTileBytes + at * kAtomBytes, &a.map_do, &bars.do_full[os], at * 64, q_row, qh, bb);
             }
         }
         __syncwarp();
@@ -174,6 +197,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc_kernel(const __grid_c
         auto issue_st = [&](int it) {  // S^T(it) = K_j Q^T
             const int qs = it % Cfg::kQStages;
             mbar_wait(&bars.q_full[qs], (it / Cfg::kQStages) & 1, &abort_flag, a.fault_word, 0x50);
+            if constexpr (RAGGED) {  // rows behind the sequence belong to the next one
+                if (q_valid(it) < kBQ) zero_tile_rows<128>(sQ + qs * Cfg::kTileBytes, Cfg::kAtoms, q_valid(it), lane);
+            }
             tc_fence_after();
             if (elect_one()) {
                 const uint64_t q_kmaj = make_smem_desc_sw128(smem_u32(sQ + qs * Cfg::kTileBytes), 0, 1024);
@@ -189,6 +215,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc_kernel(const __grid_c
         auto issue_dp = [&](int it) {  // dP^T(it) = V_j dO^T
             const int os = it % Cfg::kDoStages;
             mbar_wait(&bars.do_full[os], (it / Cfg::kDoStages) & 1, &abort_flag, a.fault_word, 0x51);
+            if constexpr (RAGGED) {
+                if (q_valid(it) < kBQ) zero_tile_rows<128>(sDO + os * Cfg::kTileBytes, Cfg::kAtoms, q_valid(it), lane);
+            }
             if (Cfg::kDqAliased && it > 0)  // the dQ partial of the previous tile sits in these columns
                 mbar_wait(&bars.dq_empty, (it - 1) & 1, &abort_flag, a.fault_word, 0x52);
             tc_fence_after();
@@ -206,6 +235,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc_kernel(const __grid_c
 
         mbar_wait(&bars.k_full, 0, &abort_flag, a.fault_word, 0x53);
         mbar_wait(&bars.v_full, 0, &abort_flag, a.fault_word, 0x54);
+        if constexpr (RAGGED) {
+            if (valid_kv < kBKV) {
+                zero_tile_rows<128>(sK, Cfg::kAtoms, valid_kv, lane);
+                zero_tile_rows<128>(sV, Cfg::kAtoms, valid_kv, lane);
+            }
+        }
         issue_st(0);
         issue_dp(0);
         for (int it = 0; it < n_it; ++it) {
@@ -285,6 +320,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc_kernel(const __grid_c
             if (tid == 0) tma_store_wait_read();  // earlier reductions have finished reading the staging tile
             named_bar_sync(2, kComputeThreads);
             uint8_t* stage = sDQ + half * kAtomBytes;
+            if (RAGGED && r >= q_valid(it)) {  // nothing is added to the rows of the next sequence, not even what is not a number
+#pragma unroll
+                for (int x = 0; x < 32; ++x) dqv[rd * 32 + x] = 0u;
+            }
 #pragma unroll
             for (int x = 0; x < 32; x += 4)
                 *reinterpret_cast<uint4*>(stage + swz128(r, x >> 2)) =
@@ -292,8 +331,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc_kernel(const __grid_c
             fence_proxy_async_smem();
             named_bar_sync(2, kComputeThreads);
             if (tid == 0) {
-                tma_reduce_add_4d(&a.map_dq_acc, sDQ, rd * 32, (jt + it) * kBQ, hh, bb);
-                tma_reduce_add_4d(&a.map_dq_acc, sDQ + kAtomBytes, D / 2 + rd * 32, (jt + it) * kBQ, hh, bb);
+                tma_reduce_add_4d(&a.map_dq_acc, sDQ, rd * 32, row0 + q_tile(it) * kBQ, q_head(it), bb);
+                tma_reduce_add_4d(&a.map_dq_acc, sDQ + kAtomBytes, D / 2 + rd * 32, row0 + q_tile(it) * kBQ, q_head(it), bb);
                 tma_store_commit();
             }
         };
@@ -303,28 +342,28 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc_kernel(const __grid_c
         // lse2[q = r], half 1 threads D[q = r], fetched one tile ahead and stored into the other buffer
         // at the END of a step, where the barrier of the dQ drain publishes them; so no barrier of their
         // own stands in front of the exponentials.
-        auto load_stat = [&](int i) -> float {
-            const int q_g = i * kBQ + r;
-            return (half == 0) ? ((q_g < a.T) ? a.lse2[stat_base + q_g] : INFINITY)  // +inf beyond T -> P = 0
-                               : ((q_g < a.T) ? a.D[stat_base + q_g] : 0.f);
+        auto load_stat = [&](int it) -> float {
+            const int q_g = q_tile(it) * kBQ + r;  // row in the sequence
+            const long long at = RAGGED ? (long long)q_head(it) * a.T + row0 + q_g : stat_base + q_g;
+            return (half == 0) ? ((q_g < len) ? a.lse2[at] : INFINITY)  // +inf beyond the end -> P = 0
+                               : ((q_g < len) ? a.D[at] : 0.f);
         };
         auto store_stat = [&](int buf, float v) {
             if (half == 0) s_lse[buf][r] = v;
             else s_D[buf][r] = v;
         };
-        store_stat(0, load_stat(jt));
-        float stat_next = (n_it > 1) ? load_stat(jt + 1) : 0.f;
+        store_stat(0, load_stat(0));
+        float stat_next = (n_it > 1) ? load_stat(1) : 0.f;
         named_bar_sync(1, kComputeThreads);
 
         for (int it = 0; it < n_it; ++it) {
-            const int i = jt + it;
             const int buf = it & 1;
 
             // ---- P^T
             mbar_wait(&bars.s_full, it & 1, &abort_flag, a.fault_word, 0x61);
             tc_fence_after();
             float p[kBQ / 2];
-            const bool diag = (i == jt);
+            const bool diag = (q_tile(it) == jt);
 #pragma unroll
             for (int cc = 0; cc < kBQ / 2; cc += 32) {
                 const int c = c_begin + cc;
@@ -401,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc_kernel(const __grid_c
             // barrier inside dq_send (or the explicit one on the first step) publishes the statistics
             if (it + 1 < n_it) {
                 store_stat(buf ^ 1, stat_next);
-                if (it + 2 < n_it) stat_next = load_stat(i + 2);
+                if (it + 2 < n_it) stat_next = load_stat(it + 2);
             }
             if (it == 0) {
                 named_bar_sync(1, kComputeThreads);
@@ -418,6 +457,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc_kernel(const __grid_c
 
         // ---- epilogue: dV and dK of this key tile
         const int kv_g = jt * kBKV + r;
+        const bool partial = RAGGED && valid_kv < kBKV;  // the rows behind the sequence are not this tile's to write
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
             const uint32_t col0 = which == 0 ? Cfg::kColDV : Cfg::kColDK;
@@ -446,18 +486,24 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc_kernel(const __grid_c
                         w.y = pack_bf16x2(__uint_as_float(v[x + 2]), __uint_as_float(v[x + 3]));
                         w.z = pack_bf16x2(__uint_as_float(v[x + 4]), __uint_as_float(v[x + 5]));
                         w.w = pack_bf16x2(__uint_as_float(v[x + 6]), __uint_as_float(v[x + 7]));
-                        *reinterpret_cast<uint4*>(atom + swz128(r, ((c & 63) + x) >> 3)) = w;
+                        if (partial) {
+                            if (r < valid_kv)
+                                *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(gout) + (long long)(row0 + kv_g) * a.ragged.out_stride +
+                                                          (long long)hh * D + c + x) = w;
+                        } else {
+                            *reinterpret_cast<uint4*>(atom + swz128(r, ((c & 63) + x) >> 3)) = w;
+                        }
                     }
                 }
             }
         }
-        if constexpr (!GRADS_F32) {
+        if (!GRADS_F32 && !partial) {
             fence_proxy_async_smem();
             named_bar_sync(1, kComputeThreads);
             if (tid == 0) {
                 for (int at = 0; at < Cfg::kAtoms; ++at) {
-                    tma_store_4d(&a.map_dv, sQ + at * kAtomBytes, at * 64, jt * kBKV, hh, bb);
-                    tma_store_4d(&a.map_dk, sQ + Cfg::kTileBytes + at * kAtomBytes, at * 64, jt * kBKV, hh, bb);
+                    tma_store_4d(&a.map_dv, sQ + at * kAtomBytes, at * 64, row0 + jt * kBKV, hh, bb);
+                    tma_store_4d(&a.map_dk, sQ + Cfg::kTileBytes + at * kAtomBytes, at * 64, row0 + jt * kBKV, hh, bb);
                 }
                 tma_store_commit();
             }
@@ -476,20 +522,6 @@ __device__ __forceinline__ float warp_sum(float x) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
     return x;
-}
-// -x/2 as three BF16 pieces (24 significant bits), twice: the 32-byte statistics row of BwdStatRows
-__device__ __forceinline__ void store_stat_row(__nv_bfloat16* dst_row, float x) {
-    const float v = -0.5f * x;
-    const __nv_bfloat16 h = __float2bfloat16_rn(v);
-    const float r1 = v - __bfloat162float(h);
-    const __nv_bfloat16 m = __float2bfloat16_rn(r1);
-    const __nv_bfloat16 l = __float2bfloat16_rn(r1 - __bfloat162float(m));
-    uint4 w;
-    w.x = uint32_t(__bfloat16_as_ushort(h)) | (uint32_t(__bfloat16_as_ushort(m)) << 16);
-    w.y = uint32_t(__bfloat16_as_ushort(l));
-    w.z = 0u, w.w = 0u;
-    reinterpret_cast<uint4*>(dst_row)[0] = w;
-    reinterpret_cast<uint4*>(dst_row)[1] = w;
 }
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
@@ -608,7 +640,7 @@ __global__ void __launch_bounds__(256) dq_convert_strided_kernel(const float* __
 template <int D, bool GRADS_F32>
 cudaError_t launch_bwd(const TcBwdArgs& a, cudaStream_t stream) {
     using Cfg = BwdCfg<D>;
-    auto kern = attn_bwd_tc_kernel<D, GRADS_F32>;
+    auto kern = attn_bwd_tc_kernel<D, GRADS_F32, false>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
     if (e != cudaSuccess) return e;
     const int n_tiles = (a.T + kBKV - 1) / kBKV;
@@ -617,6 +649,16 @@ cudaError_t launch_bwd(const TcBwdArgs& a, cudaStream_t stream) {
 }
 
 }  // namespace
+
+cudaError_t launch_attn_bwd_ragged128(const TcBwdArgs& a, cudaStream_t stream) {
+    using Cfg = BwdCfg<128>;
+    auto kern = attn_bwd_tc_kernel<128, false, true>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
+    if (e != cudaSuccess) return e;
+    const long long blocks = (long long)a.ragged.capacity * a.ragged.kv_heads;
+    if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+    return launch_pdl(kern, dim3((unsigned int)blocks), dim3(kThreads), Cfg::kSmemBytes, stream, a);
+}
 
 cudaError_t launch_attn_bwd_tc(const TcBwdArgs& a, cudaStream_t stream) {
     if (a.BH == 0 || a.T == 0) return cudaSuccess;

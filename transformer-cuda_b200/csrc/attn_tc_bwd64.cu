@@ -94,13 +94,24 @@ struct Barriers {
 
 // Position in the CTA's stream of steps. All roles walk the same stream; `n` counts work items and `g`
 // steps since the CTA started (they index the rings and give the barrier parities).
+// Packed sequences (RAGGED): an item is a key tile of one key head, its steps are the query tiles of every head of the group,
+// head by head (n_q of them per head; `sub` counts within a head).
 struct Cursor {
     int n, g;
     int bh, jt, n_it, it, hh, bb;
+    int row0, len, n_q, sub, hq;  // hq: query head of this step (= hh unless RAGGED)
     bool valid;
     __device__ __forceinline__ bool first() const { return it == 0; }
     __device__ __forceinline__ bool last() const { return it == n_it - 1; }
-    __device__ __forceinline__ int q_tile() const { return jt + it; }
+    __device__ __forceinline__ bool diagonal() const { return sub == 0; }
+    __device__ __forceinline__ int q_row() const { return row0 + (jt + sub) * kBQ; }
+    __device__ __forceinline__ int kv_row() const { return row0 + jt * kBKV; }
+    __device__ __forceinline__ int q_valid() const { return min(kBQ, len - (jt + sub) * kBQ); }   // rows that belong to the sequence
+    __device__ __forceinline__ int kv_valid() const { return min(kBKV, len - jt * kBKV); }
+    __device__ __forceinline__ void advance() {
+        ++it;
+        if (++sub == n_q) sub = 0, ++hq;
+    }
 };
 // (slab, key tile, head, batch) of work item w: ascending item index = descending length (tile-major) or slab by slab.
 // Out of line: the integer divisions are needed once per item and role, and inlined at every use they were a
@@ -123,7 +134,7 @@ __device__ __forceinline__ uint64_t make_smem_desc_sw32(uint32_t smem_addr) {
     return d;
 }
 
-template <bool GRADS_F32>
+template <bool GRADS_F32, bool RAGGED>
 __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc64_kernel(const __grid_constant__ TcBwdArgs a) {
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* sK = smem + kOffK;
@@ -140,6 +151,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc64_kernel(const __grid
     __shared__ uint32_t tmem_base_slot;
     __shared__ uint32_t abort_flag;
     __shared__ int s_item[kItemRing];
+    __shared__ int4 s_work[RAGGED ? kItemRing : 1];  // the work items behind the ids
 
     const int tid = threadIdx.x;
     const int warp = tid >> 5;
@@ -195,19 +207,27 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc64_kernel(const __grid
     pdl_wait();
 
     const int n_tiles = (a.T + kBKV - 1) / kBKV;
-    const int total_items = n_tiles * a.BH;
+    const int total_items = RAGGED ? 0 : n_tiles * a.BH;  // RAGGED: the producer reads the number of items
     // Waits: one try, then the shared out-of-line polling loop. The roles that spend most of their time waiting
     // (producer, MMA issuers, group B) sleep between polls; group A, whose waits are short, does not.
     const uint32_t sleep_ns = (warp < 4) ? 0u : 32u;
     auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t id) {
         mbar_wait_compact(bar, parity, &abort_flag, a.fault_word, id, sleep_ns);
     };
-    auto fill = [&](Cursor& c, int w) {
+    auto fill = [&](Cursor& c, int w, int slot) {
         c.valid = w >= 0;
-        if (c.valid) {
+        c.sub = 0;
+        if (RAGGED && c.valid) {
+            const int4 f = s_work[slot];
+            c.row0 = f.x, c.len = f.y, c.n_q = f.z, c.hh = w % a.ragged.kv_heads, c.bh = 0, c.bb = 0;
+            c.jt = (c.len + kBKV - 1) / kBKV - c.n_q;
+            c.n_it = c.n_q * a.ragged.group;
+            c.hq = c.hh * a.ragged.group;
+        } else if (c.valid) {
             const int4 f = decode_item(w, a.BH, a.H, n_tiles, a.tile_major_order);
             c.bh = f.x, c.jt = f.y, c.hh = f.z, c.bb = f.w;
-            c.n_it = n_tiles - c.jt;  // query tiles jt .. n_tiles-1; tiles before the diagonal are skipped
+            c.n_it = c.n_q = n_tiles - c.jt;  // query tiles jt .. n_tiles-1; tiles before the diagonal are skipped
+            c.row0 = 0, c.len = a.T, c.hq = c.hh;
         }
         c.it = 0;
     };
@@ -219,7 +239,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc64_kernel(const __grid
     // role leaves its loop at the next item boundary.
     auto next_step = [&](Cursor& c) -> bool {
         ++c.g;
-        if (c.n < 0 || ++c.it == c.n_it) {
+        if (c.n >= 0) c.advance();
+        if (c.n < 0 || c.it == c.n_it) {
             ++c.n;
             wait(&bars.item_full[c.n % kItemRing], (c.n / kItemRing) & 1, 0x70);
             const int w = *reinterpret_cast<volatile int*>(&s_item[c.n % kItemRing]);
@@ -228,12 +249,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc64_kernel(const __grid
             if (warp < 4) aborted = named_bar_or(4, kGroupThreads, mine != 0);
             else if (warp < 8) aborted = named_bar_or(5, kGroupThreads, mine != 0);
             else aborted = __any_sync(0xffffffffu, mine != 0) != 0;
-            fill(c, aborted ? -1 : w);
+            fill(c, aborted ? -1 : w, c.n % kItemRing);
         }
         return c.valid;
     };
     Cursor cur;
-    cur.n = -1, cur.g = -1, cur.it = 0, cur.n_it = 0, cur.valid = false;
+    cur.n = -1, cur.g = -1, cur.it = 0, cur.n_it = 0, cur.sub = 0, cur.n_q = 0, cur.hq = 0, cur.valid = false;
 
     constexpr uint32_t idesc_st = make_idesc_bf16(kBKV, kBQ, 0, 0);  // S^T, dP^T
     constexpr uint32_t idesc_kv = make_idesc_bf16(kBKV, kD, 0, 1);   // dV, dK: B is MN-major
@@ -249,16 +270,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc64_kernel(const __grid
             tma_prefetch_desc(&a.map_lse_ext);
             tma_prefetch_desc(&a.map_d_ext);
             int published = 0;
+            const int n_items = RAGGED ? *a.ragged.count * a.ragged.kv_heads : total_items;
             auto publish_next = [&]() {
                 int w = int(atomicAdd(a.work_counter, 1u));
-                if (w >= total_items) w = -1;
+                if (w >= n_items) w = -1;
+                if (RAGGED && w >= 0) s_work[published % kItemRing] = a.ragged.items[w / a.ragged.kv_heads];
                 s_item[published % kItemRing] = w;
                 mbar_arrive(&bars.item_full[published % kItemRing]);  // release: the slot is written before the arrival
                 ++published;
                 return w;
             };
             cur.n = 0, cur.g = 0;
-            fill(cur, publish_next());
+            fill(cur, publish_next(), 0);
             int w_next = -1;
             while (cur.valid) {
                 const int g = cur.g, n = cur.n;
@@ -267,30 +290,31 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc64_kernel(const __grid
                     const int ks = n % kKStages;
                     if (n >= kKStages) wait(&bars.k_empty[ks], (n / kKStages - 1) & 1, 0x42);
                     mbar_expect_tx(&bars.k_full[ks], kTileBytes);
-                    tma_load_4d(sK + ks * kTileBytes, &a.map_k, &bars.k_full[ks], 0, cur.jt * kBKV, cur.hh, cur.bb);
+                    tma_load_4d(sK + ks * kTileBytes, &a.map_k, &bars.k_full[ks], 0, cur.kv_row(), cur.hh, cur.bb);
                 }
                 const int qs = g % kQStages;
                 if (g >= kQStages) wait(&bars.q_empty[qs], (g / kQStages - 1) & 1, 0x40);
                 mbar_expect_tx(&bars.q_full[qs], kTileBytes + kExtBytes);
-                tma_load_4d(sQ + qs * kTileBytes, &a.map_q, &bars.q_full[qs], 0, cur.q_tile() * kBQ, cur.hh, cur.bb);
-                tma_load_4d(sLseExt + qs * kExtBytes, &a.map_lse_ext, &bars.q_full[qs], 0, cur.q_tile() * kBQ, cur.hh, cur.bb);
+                tma_load_4d(sQ + qs * kTileBytes, &a.map_q, &bars.q_full[qs], 0, cur.q_row(), cur.hq, cur.bb);
+                tma_load_4d(sLseExt + qs * kExtBytes, &a.map_lse_ext, &bars.q_full[qs], 0, cur.q_row(), cur.hq, cur.bb);
                 if (cur.first()) {
                     // V has one buffer: it is free once dP^T of the previous item's last step has retired,
                     // about one step before dP^T of this item's first step is issued
                     if (n >= 1) wait(&bars.v_empty, (n - 1) & 1, 0x43);
                     mbar_expect_tx(&bars.v_full, kTileBytes);
-                    tma_load_4d(sV, &a.map_v, &bars.v_full, 0, cur.jt * kBKV, cur.hh, cur.bb);
+                    tma_load_4d(sV, &a.map_v, &bars.v_full, 0, cur.kv_row(), cur.hh, cur.bb);
                 }
                 const int os = g % kDoStages;
                 if (g >= kDoStages) wait(&bars.do_empty[os], (g / kDoStages - 1) & 1, 0x41);
                 mbar_expect_tx(&bars.do_full[os], kTileBytes + kExtBytes);
-                tma_load_4d(sDO + os * kTileBytes, &a.map_do, &bars.do_full[os], 0, cur.q_tile() * kBQ, cur.hh, cur.bb);
-                tma_load_4d(sDExt + os * kExtBytes, &a.map_d_ext, &bars.do_full[os], 0, cur.q_tile() * kBQ, cur.hh, cur.bb);
+                tma_load_4d(sDO + os * kTileBytes, &a.map_do, &bars.do_full[os], 0, cur.q_row(), cur.hq, cur.bb);
+                tma_load_4d(sDExt + os * kExtBytes, &a.map_d_ext, &bars.do_full[os], 0, cur.q_row(), cur.hq, cur.bb);
                 // next step of the stream (the producer decodes its own published ids, no ring wait)
                 ++cur.g;
-                if (++cur.it == cur.n_it) {
+                cur.advance();
+                if (cur.it == cur.n_it) {
                     ++cur.n;
-                    fill(cur, abort_flag ? -1 : w_next);
+                    fill(cur, abort_flag ? -1 : w_next, cur.n % kItemRing);
                 }
             }
         }
@@ -304,6 +328,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc64_kernel(const __grid
             if (g > 0) wait(&bars.s_free, (g - 1) & 1, 0x59);
             if (cur.first()) wait(&bars.k_full[ks], (cur.n / kKStages) & 1, 0x53);
             wait(&bars.q_full[qs], (g / kQStages) & 1, 0x50);
+            if constexpr (RAGGED) {  // rows behind the sequence belong to the next one: as if they were not there (zeros)
+                if (cur.first() && cur.kv_valid() < kBKV) zero_tile_rows<128>(sK + ks * kTileBytes, 1, cur.kv_valid(), lane);
+                if (cur.q_valid() < kBQ) {
+                    zero_tile_rows<128>(sQ + qs * kTileBytes, 1, cur.q_valid(), lane);
+                    zero_tile_rows<32>(sLseExt + qs * kExtBytes, 1, cur.q_valid(), lane);
+                }
+            }
             tc_fence_after();
             if (lane == 0) T64(2, g, 0);
             if (elect_one()) {
@@ -328,6 +359,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc64_kernel(const __grid
             if (g > 0) wait(&bars.dp_free, (g - 1) & 1, 0x5A);
             if (cur.first()) wait(&bars.v_full, n & 1, 0x54);
             wait(&bars.do_full[os], (g / kDoStages) & 1, 0x51);
+            if constexpr (RAGGED) {
+                if (cur.first() && cur.kv_valid() < kBKV) zero_tile_rows<128>(sV, 1, cur.kv_valid(), lane);
+                if (cur.q_valid() < kBQ) {
+                    zero_tile_rows<128>(sDO + os * kTileBytes, 1, cur.q_valid(), lane);
+                    zero_tile_rows<32>(sDExt + os * kExtBytes, 1, cur.q_valid(), lane);
+                }
+            }
             tc_fence_after();
             if (lane == 0) T64(3, g, 0);
             if (elect_one()) {
@@ -403,7 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc64_kernel(const __grid
         const float scale_log2 = a.scale * kLog2e;
         while (next_step(cur)) {
             const int g = cur.g;
-            const bool diag = cur.first();  // the diagonal tile of this item: query column c is masked for key row r when c < r
+            const bool diag = cur.diagonal();  // the diagonal tile of this item (of each of its heads): query column c is masked for key row r when c < r
             if (r == 0) T64(0, g, 0);
             wait(&bars.s_full, g & 1, 0x61);
             tc_fence_after();
@@ -563,6 +601,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc64_kernel(const __grid
                 if (leader) tma_store_wait_read();  // earlier reductions have finished reading the staging tile
                 named_bar_sync(2, kGroupThreads);
                 if (leader) T64(1, prev.g + 1, 6);
+                if (RAGGED && r >= prev.q_valid()) {  // nothing is added to the rows of the next sequence, not even what is not a number
+#pragma unroll
+                    for (int x = 0; x < kD; ++x) dq[x] = 0u;
+                }
                 if constexpr (GRADS_F32) {  // the accumulator is the caller's dq: no conversion pass will apply the scale
 #pragma unroll
                     for (int x = 0; x < kD; ++x) dq[x] = __float_as_uint(__uint_as_float(dq[x]) * a.scale);
@@ -577,8 +619,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc64_kernel(const __grid
                 named_bar_sync(2, kGroupThreads);
                 if (leader) T64(1, prev.g + 1, 7);
                 if (leader) {
-                    tma_reduce_add_4d(&a.map_dq_acc, sStage, 0, prev.q_tile() * kBQ, prev.hh, prev.bb);
-                    tma_reduce_add_4d(&a.map_dq_acc, sStage + kTileBytes, 32, prev.q_tile() * kBQ, prev.hh, prev.bb);
+                    tma_reduce_add_4d(&a.map_dq_acc, sStage, 0, prev.q_row(), prev.hq, prev.bb);
+                    tma_reduce_add_4d(&a.map_dq_acc, sStage + kTileBytes, 32, prev.q_row(), prev.hq, prev.bb);
                     tma_store_commit();
                 }
                 if (prev.last()) {
@@ -586,7 +628,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc64_kernel(const __grid
                     // global. A thread owns one key row: 128 bytes of BF16 (256 of FP32) per tensor, 16-byte stores.
                     wait(&bars.dv_done, prev.n & 1, 0x65);  // the dV MMAs come from another thread than the dQ ones
                     tc_fence_after();
-                    const int kv_g = prev.jt * kBKV + r;
+                    const int kv_g = prev.kv_row() + r;
+                    const bool in_range = RAGGED ? r < prev.kv_valid() : kv_g < a.T;
 #pragma unroll 1
                     for (int which = 0; which < 2; ++which) {
                         uint32_t acc[kD];
@@ -598,7 +641,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc64_kernel(const __grid
                             mbar_arrive(&bars.acc_free);
                         }
                         const float mul = (which == 1) ? a.scale : 1.0f;  // dK: dS was left unscaled
-                        if (kv_g < a.T) {
+                        if (in_range) {
                             if constexpr (GRADS_F32) {
                                 float* dst = reinterpret_cast<float*>(which == 0 ? a.dv : a.dk) + ((long long)prev.bh * a.T + kv_g) * kD;
 #pragma unroll
@@ -638,7 +681,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc64_kernel(const __grid
 
 template <bool GRADS_F32>
 cudaError_t launch_bwd64(const TcBwdArgs& a, cudaStream_t stream) {
-    auto kern = attn_bwd_tc64_kernel<GRADS_F32>;
+    auto kern = attn_bwd_tc64_kernel<GRADS_F32, false>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
     if (e != cudaSuccess) return e;
     int dev = 0, sms = 0;
@@ -650,6 +693,18 @@ cudaError_t launch_bwd64(const TcBwdArgs& a, cudaStream_t stream) {
 }
 
 }  // namespace
+
+cudaError_t launch_attn_bwd_ragged64(const TcBwdArgs& a, cudaStream_t stream) {
+    auto kern = attn_bwd_tc64_kernel<false, true>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    if (e != cudaSuccess) return e;
+    int dev = 0, sms = 0;
+    if ((e = cudaGetDevice(&dev)) != cudaSuccess) return e;
+    if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
+    const long long items = (long long)a.ragged.capacity * a.ragged.kv_heads;
+    if (items > 0x7fffffffLL) return cudaErrorInvalidValue;
+    return launch_pdl(kern, dim3((unsigned int)(items < sms ? items : sms)), dim3(kThreads), kSmemBytes, stream, a);
+}
 
 cudaError_t launch_attn_bwd_tc64(const TcBwdArgs& a, cudaStream_t stream) {
     if (a.BH == 0 || a.T == 0) return cudaSuccess;

@@ -68,7 +68,8 @@ struct FwdBarriers {
     uint64_t o_done;
 };
 
-template <int D, bool OUT_F32>
+// RAGGED: packed sequences with grouped heads; the tile, its sequence and its rows come from a work item (RaggedWork).
+template <int D, bool OUT_F32, bool RAGGED>
 __global__ void __launch_bounds__(kThreads, 2) attn_fwd_tc_short_kernel(const __grid_constant__ TcFwdArgs a) {
     using Cfg = FwdCfg<D>;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -88,10 +89,13 @@ __global__ void __launch_bounds__(kThreads, 2) attn_fwd_tc_short_kernel(const __
     const int n_q_tiles = (a.T + kBM - 1) / kBM;
     // CTA order: the last query tile of a slab is the longest. Longest-first across all slabs when the
     // problem fits in L2 (shortest tail), else slab by slab (resident CTAs share K/V tiles in L2).
-    const int bh = a.tile_major_order ? int(blockIdx.x % a.BH) : int(blockIdx.x / n_q_tiles);
-    const int qt = n_q_tiles - 1 - (a.tile_major_order ? int(blockIdx.x / a.BH) : int(blockIdx.x % n_q_tiles));
-    const int hh = bh % a.H, bb = bh / a.H;  // head and batch coordinates of the 4-D tensor maps
-    const int n_kv = qt + 1;                                  // key tiles 0..qt; qt is the diagonal tile
+    int bh = 0, qt = 0, hh = 0, bb = 0, hk = 0;  // hh, bb: head and batch coordinates of the 4-D tensor maps; hk: key head
+    int row0 = 0, valid = kBM;                   // RAGGED: first row of the sequence, rows of this tile that belong to it
+    if constexpr (!RAGGED) {
+        bh = a.tile_major_order ? int(blockIdx.x % a.BH) : int(blockIdx.x / n_q_tiles);
+        qt = n_q_tiles - 1 - (a.tile_major_order ? int(blockIdx.x / a.BH) : int(blockIdx.x % n_q_tiles));
+        hh = bh % a.H, bb = bh / a.H, hk = hh;
+    }
 
     if (tid == 0) {
         mbar_init(&bars.q_full, 1);
@@ -120,6 +124,18 @@ __global__ void __launch_bounds__(kThreads, 2) attn_fwd_tc_short_kernel(const __
     // barriers, TMEM and the tensor maps are set up: from here on global memory is touched, so wait for the
     // kernel in front of this one in the stream (returns at once for an ordinary launch)
     pdl_wait();
+    if constexpr (RAGGED) {  // the heads of one tile are neighbours: those of a group read the same key tiles
+        const int item = int(blockIdx.x / unsigned(a.H));
+        if (item >= *a.ragged.count) {
+            __syncthreads();
+            if (warp == 4) tmem_dealloc(tmem, Cfg::kTmemCols);
+            return;
+        }
+        const int4 w = a.ragged.items[item];
+        bh = hh = int(blockIdx.x % unsigned(a.H)), hk = hh / a.ragged.group;
+        row0 = w.x, qt = w.z - 1, valid = min(kBM, w.y - qt * kBM);
+    }
+    const int n_kv = qt + 1;  // key tiles 0..qt; qt is the diagonal tile
 
     if (warp == 4) {
         // ------------------------------------------------------------ TMA producer
@@ -129,18 +145,18 @@ __global__ void __launch_bounds__(kThreads, 2) attn_fwd_tc_short_kernel(const __
             tma_prefetch_desc(&a.map_v);
             mbar_expect_tx(&bars.q_full, Cfg::kTileBytes);
             for (int at = 0; at < Cfg::kAtoms; ++at)
-                tma_load_4d(sQ + at * kAtomBytes, &a.map_q, &bars.q_full, at * 64, qt * kBM, hh, bb);
+                tma_load_4d(sQ + at * kAtomBytes, &a.map_q, &bars.q_full, at * 64, row0 + qt * kBM, hh, bb);
             for (int j = 0; j < n_kv; ++j) {
                 const int s = j % Cfg::kStages;
                 const int round = j / Cfg::kStages;
                 if (round > 0) mbar_wait(&bars.k_empty[s], (round - 1) & 1, &abort_flag, a.fault_word, 0x10);
                 mbar_expect_tx(&bars.k_full[s], Cfg::kTileBytes);
                 for (int at = 0; at < Cfg::kAtoms; ++at)
-                    tma_load_4d(sK + s * Cfg::kTileBytes + at * kAtomBytes, &a.map_k, &bars.k_full[s], at * 64, j * kBN, hh, bb);
+                    tma_load_4d(sK + s * Cfg::kTileBytes + at * kAtomBytes, &a.map_k, &bars.k_full[s], at * 64, row0 + j * kBN, hk, bb);
                 if (round > 0) mbar_wait(&bars.v_empty[s], (round - 1) & 1, &abort_flag, a.fault_word, 0x11);
                 mbar_expect_tx(&bars.v_full[s], Cfg::kTileBytes);
                 for (int at = 0; at < Cfg::kAtoms; ++at)
-                    tma_load_4d(sV + s * Cfg::kTileBytes + at * kAtomBytes, &a.map_v, &bars.v_full[s], at * 64, j * kBN, hh, bb);
+                    tma_load_4d(sV + s * Cfg::kTileBytes + at * kAtomBytes, &a.map_v, &bars.v_full[s], at * 64, row0 + j * kBN, hk, bb);
             }
         }
         __syncwarp();
@@ -182,6 +198,9 @@ __global__ void __launch_bounds__(kThreads, 2) attn_fwd_tc_short_kernel(const __
             }
             // O += P_j V_j
             mbar_wait(&bars.v_full[s], ring_phase, &abort_flag, a.fault_word, 0x22);
+            if constexpr (RAGGED) {  // keys behind the sequence have P = 0, whatever their values hold
+                if (j == qt && valid < kBN) zero_tile_rows<128>(sV + s * Cfg::kTileBytes, Cfg::kAtoms, valid, lane);
+            }
             mbar_wait(&bars.p_full, j & 1, &abort_flag, a.fault_word, 0x23);
             tc_fence_after();
             if (elect_one()) {
@@ -280,9 +299,10 @@ __global__ void __launch_bounds__(kThreads, 2) attn_fwd_tc_short_kernel(const __
         mbar_wait(&bars.o_done, (n_kv - 1) & 1, &abort_flag, a.fault_word, 0x32);
         tc_fence_after();
         const float inv_l = 1.0f / l_run;
-        const int row_g = qt * kBM + r;
+        const int row_g = row0 + qt * kBM + r;
+        const bool in_range = RAGGED ? r < valid : row_g < a.T;
         const long long stat_idx = (long long)bh * a.T + row_g;
-        if (row_g < a.T) {
+        if (in_range) {
             // exported statistics are relative to the true row maximum
             if (a.m_out) a.m_out[stat_idx] = m_true * kLn2;
             if (a.l_out) a.l_out[stat_idx] = l_run * exp2f(m_ref - m_true);
@@ -294,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_fwd_tc_short_kernel(const __
             tmem_ld32(tmem_addr(tmem, lane_base, Cfg::kColO + c), ov);
             tmem_wait_ld();
             if constexpr (OUT_F32) {
-                if (row_g < a.T) {
+                if (in_range) {
                     float* dst = reinterpret_cast<float*>(a.out) + ((long long)bh * a.T + row_g) * D + c;
 #pragma unroll
                     for (int i = 0; i < 32; i += 4)
@@ -312,15 +332,21 @@ __global__ void __launch_bounds__(kThreads, 2) attn_fwd_tc_short_kernel(const __
                     w.y = pack_bf16x2(__uint_as_float(ov[i + 2]) * inv_l, __uint_as_float(ov[i + 3]) * inv_l);
                     w.z = pack_bf16x2(__uint_as_float(ov[i + 4]) * inv_l, __uint_as_float(ov[i + 5]) * inv_l);
                     w.w = pack_bf16x2(__uint_as_float(ov[i + 6]) * inv_l, __uint_as_float(ov[i + 7]) * inv_l);
-                    *reinterpret_cast<uint4*>(atom + swz128(r, ((c & 63) + i) >> 3)) = w;
+                    if (RAGGED && valid < kBM) {  // the rows behind the sequence are not this tile's to write
+                        if (in_range)
+                            *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(a.out) + (long long)row_g * a.ragged.out_stride +
+                                                      (long long)hh * D + c + i) = w;
+                    } else {
+                        *reinterpret_cast<uint4*>(atom + swz128(r, ((c & 63) + i) >> 3)) = w;
+                    }
                 }
             }
         }
-        if constexpr (!OUT_F32) {
+        if (!OUT_F32 && !(RAGGED && valid < kBM)) {
             fence_proxy_async_smem();
             named_bar_sync(1, kSoftmaxThreads);
             if (tid == 0) {
-                for (int at = 0; at < Cfg::kAtoms; ++at) tma_store_4d(&a.map_o, sQ + at * kAtomBytes, at * 64, qt * kBM, hh, bb);
+                for (int at = 0; at < Cfg::kAtoms; ++at) tma_store_4d(&a.map_o, sQ + at * kAtomBytes, at * 64, row0 + qt * kBM, hh, bb);
                 tma_store_commit();
                 tma_store_wait_read();  // the staging tile must outlive the bulk read; the write completes with the grid
             }
@@ -334,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_fwd_tc_short_kernel(const __
 template <int D, bool OUT_F32>
 cudaError_t launch_fwd_short(const TcFwdArgs& a, cudaStream_t stream) {
     using Cfg = FwdCfg<D>;
-    auto kern = attn_fwd_tc_short_kernel<D, OUT_F32>;
+    auto kern = attn_fwd_tc_short_kernel<D, OUT_F32, false>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
     if (e != cudaSuccess) return e;
     const int n_q_tiles = (a.T + kBM - 1) / kBM;
@@ -342,7 +368,24 @@ cudaError_t launch_fwd_short(const TcFwdArgs& a, cudaStream_t stream) {
     return launch_pdl(kern, dim3((unsigned int)blocks), dim3(kThreads), Cfg::kSmemBytes, stream, a);
 }
 
+template <int D>
+cudaError_t launch_fwd_ragged(const TcFwdArgs& a, cudaStream_t stream) {
+    using Cfg = FwdCfg<D>;
+    auto kern = attn_fwd_tc_short_kernel<D, false, true>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
+    if (e != cudaSuccess) return e;
+    const long long blocks = (long long)a.ragged.capacity * a.H;
+    if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+    return launch_pdl(kern, dim3((unsigned int)blocks), dim3(kThreads), Cfg::kSmemBytes, stream, a);
+}
+
 }  // namespace
+
+cudaError_t launch_attn_fwd_ragged(const TcFwdArgs& a, cudaStream_t stream) {
+    if (a.d == 64) return launch_fwd_ragged<64>(a, stream);
+    if (a.d == 128) return launch_fwd_ragged<128>(a, stream);
+    return cudaErrorInvalidValue;
+}
 
 cudaError_t launch_attn_fwd_tc_short(const TcFwdArgs& a, cudaStream_t stream) {
     if (a.BH == 0 || a.T == 0) return cudaSuccess;

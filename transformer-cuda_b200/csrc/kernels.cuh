@@ -83,6 +83,23 @@ cudaError_t launch_attn_bwd_f32_tiled(const float* q, const float* k, const floa
 // ------------------------------------------------------------------ attn_tc_fwd.cu / attn_tc_bwd.cu (tcgen05)
 // Tensor maps are 4-D (d, T, H, B) with free T / H / B strides, box 64 x 128 x 1 x 1 (FP32: 32 x 128 x 1 x 1) and the
 // 128-byte swizzle; slab bh = b*H + h. (B, H, T, d) slabs and the interleaved (B, T, 3*H*d) buffer differ only in strides.
+
+// Packed sequences: every tensor is (T, heads, d) with T the rows of all sequences, i.e. maps with B = 1; statistics are (H, T).
+// A work item is one 128-row tile of one sequence: {first row of the sequence, its length, tiles, 0} where `tiles` is how many
+// tiles the item walks per head. The forward's item is query tile `tiles - 1` (key tiles 0 .. tiles - 1), the backward's key
+// tile n - tiles of the sequence's n (query tiles from there to the last). Items are in descending order of `tiles`.
+struct RaggedWork {
+    const int4* items;
+    const int* count;     // number of items (device)
+    int capacity;         // upper bound of it known to the host
+    int group;            // query heads per key head
+    int kv_heads;
+    long long out_stride; // element stride between rows of `out` (forward) or of dk and dv (backward)
+};
+// Writes items and count from the n + 1 offsets (device), clipped to [0, T], and clears *counter.
+cudaError_t launch_ragged_plan(const int* offsets, int n, int T, int4* items, int* count, int capacity, unsigned int* counter,
+                               cudaStream_t stream);
+
 struct TcFwdArgs {
     CUtensorMap map_q, map_k, map_v, map_o;  // BF16
     void* out;                               // BF16 or FP32 (BH, T, d), selected by out_is_f32
@@ -95,9 +112,11 @@ struct TcFwdArgs {
     int tile_major_order;  // 1: CTAs ordered longest tile first across all slabs; 0: slab by slab
     float scale;
     unsigned int* fault_word;
+    RaggedWork ragged;     // packed sequences (launch_attn_fwd_ragged), else unused
 };
 cudaError_t launch_attn_fwd_tc(const TcFwdArgs& a, cudaStream_t stream);        // picks the variant by T
 cudaError_t launch_attn_fwd_tc_short(const TcFwdArgs& a, cudaStream_t stream);  // two CTAs per SM (d = 64; d = 128 up to T = 4096)
+cudaError_t launch_attn_fwd_ragged(const TcFwdArgs& a, cudaStream_t stream);    // packed sequences, BF16 output
 
 struct TcBwdArgs {
     CUtensorMap map_q, map_k, map_v, map_do;  // BF16
@@ -118,6 +137,7 @@ struct TcBwdArgs {
     unsigned int* work_counter;          // device word, zero at launch: next work item to hand out
     long long grad_lt, grad_lh, grad_lb; // element strides (row, head, batch) of the BF16 dk / dv tensors
     CUtensorMap map_lse_ext, map_d_ext;  // BF16 (BH*T, 16) statistics rows written by the pre-pass (see BwdStatRows)
+    RaggedWork ragged;                   // packed sequences (launch_attn_bwd_ragged*), else unused
 };
 // Statistics rows for the persistent head-dim-64 kernel: per query row 16 BF16 = two identical 16-byte halves
 // [hi, mid, lo, 0, 0, 0, 0, 0] with hi + mid + lo = -x/2 to 24 significant bits, x = lse/scale (lse_ext) or D (d_ext).
@@ -131,6 +151,8 @@ struct BwdStatRows {
 // kernel of attn_tc_bwd64.cu.
 cudaError_t launch_attn_bwd_tc(const TcBwdArgs& a, cudaStream_t stream);
 cudaError_t launch_attn_bwd_tc64(const TcBwdArgs& a, cudaStream_t stream);
+cudaError_t launch_attn_bwd_ragged128(const TcBwdArgs& a, cudaStream_t stream);  // packed sequences, d = 128
+cudaError_t launch_attn_bwd_ragged64(const TcBwdArgs& a, cudaStream_t stream);   // packed sequences, d = 64
 
 // Backward pre-pass: D = rowsum(dO*O) and lse2 = (m + log l) * log2(e) or lse * log2(e).
 // TIn is float or __nv_bfloat16. Exactly one of (m,l) / lse is given. If `zero` is not null the
@@ -152,6 +174,33 @@ cudaError_t launch_dq_convert_strided(const float* dq_acc, __nv_bfloat16* dq, lo
                                       long long lt, long long lh, long long lb, cudaStream_t stream, float scale = 1.0f);
 // dq (BF16) = dq_acc (FP32) * scale, elementwise.
 cudaError_t launch_dq_convert(const float* dq_acc, __nv_bfloat16* dq, long long n, cudaStream_t stream, float scale = 1.0f);
+
+// ------------------------------------------------------------------ attn_ragged.cu (passes around the kernels for packed sequences)
+// D, lse2 (and, with ext, the statistics rows) of all T x H rows, (H, T); clears the (T, H, d) FP32 accumulator dq_acc.
+cudaError_t launch_ragged_prepass(const __nv_bfloat16* o, long long o_stride, const __nv_bfloat16* dO, long long do_stride,
+                                  const float* lse, float* D, float* lse2, float* dq_acc, int T, int H, int d, BwdStatRows ext,
+                                  cudaStream_t stream);
+// dq (BF16 rows at dq_stride) = dq_acc * scale for the rows offsets[0] .. offsets[n] (clipped to [0, T]); others keep their values.
+cudaError_t launch_ragged_dq_convert(const float* dq_acc, __nv_bfloat16* dq, long long dq_stride, const int* offsets, int n, int T,
+                                     int H, int d, float scale, cudaStream_t stream);
+
+// ------------------------------------------------------------------ attn_decode.cu (one query token per sequence)
+struct DecodeArgs {
+    const __nv_bfloat16 *q, *k, *v;
+    const int* lengths;
+    __nv_bfloat16* out;             // (B, H, d)
+    float* lse;                     // (B, H)
+    float* part_o;                  // splits > 1: (B, H, splits, d) sums and (B, H, splits, 2) maximum and sum
+    float* part_ml;
+    int B, T, H, Hkv, d;
+    long long q_stride;             // elements from sequence to sequence
+    long long k_batch, k_row, k_head, v_batch, v_row, v_head;
+    float scale;
+    int splits;                     // decode_splits()
+    int G, head_blocks;             // filled in by the launcher
+};
+int decode_splits(int B, int T, int H, int Hkv);
+cudaError_t launch_attn_decode(DecodeArgs a, cudaStream_t stream);
 
 // ------------------------------------------------------------------ wait_selftest.cu
 // One CTA waits (with a limit of a few thousand polls) on a barrier nothing arrives on, so that the wait gives up and

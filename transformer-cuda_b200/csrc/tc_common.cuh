@@ -289,6 +289,19 @@ __device__ __forceinline__ uint32_t swz128(uint32_t row, uint32_t chunk) {
     return row * 128u + ((chunk ^ (row & 7u)) << 4);
 }
 
+// Clears rows first..127 of a tile of 128-row boxes whose rows are kRowBytes long (32 or 128, any swizzle up to that: a swizzle
+// moves 16-byte chunks inside a row only). Executed by one warp; makes the zeros visible to the tensor core. Packed sequences
+// need it where a tile reaches past the end of one: the rows behind belong to the next sequence, or to nobody, and a NaN
+// there would survive the product with a masked probability.
+template <int kRowBytes>
+__device__ __forceinline__ void zero_tile_rows(uint8_t* tile, int boxes, int first, int lane) {
+    for (int b = 0; b < boxes; ++b)
+        for (int x = first * kRowBytes + lane * 16; x < 128 * kRowBytes; x += 512)
+            *reinterpret_cast<uint4*>(tile + b * 128 * kRowBytes + x) = make_uint4(0u, 0u, 0u, 0u);
+    fence_proxy_async_smem();
+    __syncwarp();
+}
+
 // TMEM address = (lane << 16) | column.
 __device__ __forceinline__ uint32_t tmem_addr(uint32_t base, uint32_t lane, uint32_t col) {
     return base + (lane << 16) + col;
@@ -349,6 +362,21 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
+}
+
+// -x/2 as three BF16 pieces (24 significant bits), twice: the 32-byte statistics row of BwdStatRows
+__device__ __forceinline__ void store_stat_row(__nv_bfloat16* dst_row, float x) {
+    const float v = -0.5f * x;
+    const __nv_bfloat16 h = __float2bfloat16_rn(v);
+    const float r1 = v - __bfloat162float(h);
+    const __nv_bfloat16 m = __float2bfloat16_rn(r1);
+    const __nv_bfloat16 l = __float2bfloat16_rn(r1 - __bfloat162float(m));
+    uint4 w;
+    w.x = uint32_t(__bfloat16_as_ushort(h)) | (uint32_t(__bfloat16_as_ushort(m)) << 16);
+    w.y = uint32_t(__bfloat16_as_ushort(l));
+    w.z = 0u, w.w = 0u;
+    reinterpret_cast<uint4*>(dst_row)[0] = w;
+    reinterpret_cast<uint4*>(dst_row)[1] = w;
 }
 
 // Elementwise product of two packed bf16x2 words.
