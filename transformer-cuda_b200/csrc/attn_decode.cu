@@ -2,16 +2,19 @@
 //
 //   out[b, h] = softmax(scale * q[b, h] K[b, :len_b, h / G]^T) V[b, :len_b, h / G],   G = H / Hkv query heads to a key head
 //
-// Every key and value is read once and used for G heads only, so the bound is HBM and nothing needs staging: the operands of
-// the products go from global memory straight into the registers of mma.sync m16n8k16, whose 16 rows are the heads of a group.
+// Every key and value is read once and used for G heads only, so the bound is HBM, and what counts is bytes in flight and the shape
+// of the requests. cp.async brings the rows of the next steps into shared memory, three steps per warp (192 KB per SM), a row by
+// neighbouring lanes: the first version loaded every lane's 16-byte operands straight into registers (64 bytes of a row per
+// request) and stayed at 4.7 TB/s however much was in flight; whole rows per request reach 5.8 TB/s. The operands of mma.sync
+// m16n8k16, whose 16 rows are the heads of a group, are then read with 16-byte loads:
 //   * Q K^T: the contraction index may be permuted freely as long as both operands agree, so lane (g, t) = (lane / 4, lane % 4)
-//     takes 16 contiguous bytes of key g (dims 32c + 8t .. +7), which are its B fragments of two steps; Q is read the same way.
+//     takes 16 contiguous bytes of key g (dims 32c + 8t .. +7), which are its B fragments of two products; Q is read the same way.
 //   * P V: the scores' accumulator layout is the A layout of the next product (keys 2t, 2t+1 and 2t+8, 2t+9 of 16). Lane (g, t)
 //     takes dims 64e + 8g .. +7 of those four keys, 16 bytes each; pairs of keys are interleaved with a byte permute, and the
 //     output columns are permuted with it: lane (g, t) ends with dims 64e + 16t .. +15 of head g.
 // Groups of up to 8 heads leave rows 8-15 of the products empty (their accumulators are never kept).
 //
-// A CTA of eight warps takes one split of one (sequence, key head); warp w takes the 16-key tiles w, w + 8, ... of it with its
+// A CTA of four warps takes one split of one (sequence, key head); warp w takes the 16-key tiles w, w + 4, ... of it with its
 // own running maximum and sum, and the warps meet in shared memory. The splits of a sequence are equal parts of ITS length
 // (read on the device), so a long capacity with short lengths costs nothing. With more than one split the parts go to a
 // workspace and a second kernel joins them in a fixed order: results do not depend on timing.
@@ -21,37 +24,41 @@
 namespace b200attn {
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kTile = 16;                      // keys per warp and step
-constexpr int kMinChunk = kTile * kWarps;      // keys of a split, at least: one tile for every warp
+constexpr int kStages = 3;                     // steps of K and V in flight per warp
+constexpr int kRound = kTile * kWarps;         // keys of a CTA and step; a split is a multiple of it
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kNoKey = -1e30f;               // running maximum before the first key (finite: differences of it are numbers)
 
 __device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Streaming 16-byte load (every key and value is read once).
-__device__ __forceinline__ uint4 load_stream(const __nv_bfloat16* p) {
-    uint4 w;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "l"(p));
-    return w;
+// Asynchronous 16-byte copy to shared memory; zeros when `live` is false (nothing is read then).
+__device__ __forceinline__ void copy16(uint4* dst, const __nv_bfloat16* src, bool live) {
+    asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
 }
 
 // Keys of one split of a sequence of `len` keys (the last one may be shorter; splits past the end are empty).
 __device__ __forceinline__ int chunk_of(int len, int splits) {
     const int c = (len + splits - 1) / splits;
-    return max(kMinChunk, (c + kTile - 1) / kTile * kTile);
+    return max(1, (c + kRound - 1) / kRound) * kRound;
 }
 __device__ __forceinline__ int length_of(const DecodeArgs& a, int b) { return min(max(a.lengths[b], 0), a.T); }
 
 // R = 8: the block of heads has at most 8; R = 16: up to 16.
 template <int D, int R>
-__global__ void __launch_bounds__(kThreads) attn_decode_kernel(const DecodeArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) attn_decode_kernel(const DecodeArgs a) {
     constexpr int kRowsPerLane = R / 8;  // head g, and head g + 8
     constexpr int kSets = D / 32;        // 16-byte pieces of a key per lane
     constexpr int kHalves = D / 64;
@@ -61,8 +68,8 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kernel(const DecodeArgs 
 
     pdl_launch_dependents();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int split = blockIdx.x, b = blockIdx.z;
-    const int kvh = blockIdx.y / a.head_blocks, block = blockIdx.y % a.head_blocks;
+    const int split = blockIdx.y, b = blockIdx.z;
+    const int kvh = blockIdx.x / a.head_blocks, block = blockIdx.x % a.head_blocks;
     const int h0 = kvh * a.G + block * R;          // first query head of this CTA
     const int rows = min(R, a.G - block * R);      // heads of it
     pdl_wait();
@@ -99,40 +106,66 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kernel(const DecodeArgs 
 #pragma unroll
     for (int x = 0; x < kRowsPerLane; ++x) m[x] = kNoKey, l[x] = 0.f;
 
-    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-    uint4 kf[2][kSets];
-    auto load_keys = [&](int k0) {
+    // A stage of this warp: 16 rows of K, then 16 rows of V, of kChunks 16-byte chunks. A row is copied by neighbouring lanes (whole
+    // 128-byte lines go to L2). Chunks are exchanged inside a row so that eight lanes that read together meet eight bank groups:
+    // K rows g, g + 1 at chunks 4c + t, V rows 2t at chunks 8e + g.
+    constexpr int kChunks = D / 8, kRowsPerCopy = 32 / kChunks, kCopies = kTile / kRowsPerCopy;
+    constexpr int kStage = 2 * kTile * kChunks;  // in 16-byte chunks
+    uint4* ring = reinterpret_cast<uint4*>(s_sums) + warp * kStages * kStage;
+    const int crow = lane / kChunks, cchunk = lane % kChunks;  // this lane's row and chunk of a copy's first rows
+    int k_next = begin + warp * kTile;
+    const __nv_bfloat16* kp = kbase + (long long)(k_next + crow) * a.k_row + cchunk * 8;
+    const __nv_bfloat16* vp = vbase + (long long)(k_next + crow) * a.v_row + cchunk * 8;
+    auto issue = [&](int stage) {
+        if (k_next < end) {
+            uint4* at = ring + stage * kStage;
+            const bool whole = k_next + kTile <= end;
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            const int key = k0 + 8 * n + g;
-            const __nv_bfloat16* p = kbase + (long long)key * a.k_row + t * 8;
-#pragma unroll
-            for (int c = 0; c < kSets; ++c) kf[n][c] = key < end ? load_stream(p + c * 32) : zero;
-        }
-    };
-    int k0 = begin + warp * kTile;
-    if (k0 < end) load_keys(k0);
-    for (; k0 < end; k0 += kTile * kWarps) {
-        uint4 vf[kHalves][4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int key = k0 + 2 * t + (i & 1) + 8 * (i >> 1);
-            const __nv_bfloat16* p = vbase + (long long)key * a.v_row + g * 8;
-#pragma unroll
-            for (int e = 0; e < kHalves; ++e) vf[e][i] = key < end ? load_stream(p + e * 64) : zero;
-        }
-        float s[2][4];
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-#pragma unroll
-            for (int x = 0; x < 4; ++x) s[n][x] = 0.f;
-#pragma unroll
-            for (int c = 0; c < kSets; ++c) {
-                mma16816(s[n], qf[c][0], kf[n][c].x, kf[n][c].y);
-                mma16816(s[n], qf[c][1], kf[n][c].z, kf[n][c].w);
+            for (int i = 0; i < kCopies; ++i) {
+                const int row = i * kRowsPerCopy + crow;
+                const bool live = whole || k_next + row < end;
+                copy16(at + row * kChunks + (cchunk ^ ((row & 1) << 2)), live ? kp + i * kRowsPerCopy * a.k_row : kbase, live);
             }
+#pragma unroll
+            for (int i = 0; i < kCopies; ++i) {
+                const int row = i * kRowsPerCopy + crow;
+                const bool live = whole || k_next + row < end;
+                copy16(at + (kTile + row) * kChunks + (cchunk ^ (((row >> 1) & 3) << 1)), live ? vp + i * kRowsPerCopy * a.v_row : vbase, live);
+            }
+            k_next += kRound, kp += kRound * a.k_row, vp += kRound * a.v_row;
         }
-        if (k0 + kTile * kWarps < end) load_keys(k0 + kTile * kWarps);
+        copy_commit();  // also where there is nothing left: the groups are counted
+    };
+    int k0 = begin + warp * kTile, stage = 0;
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) issue(i);
+    for (; k0 < end; k0 += kRound) {
+        copy_wait<kStages - 2>();
+        __syncwarp();  // every lane's copies of this stage are there, and the stage before has been read by all
+        issue(stage == 0 ? kStages - 1 : stage - 1);
+        const uint4* at = ring + stage * kStage;
+        stage = stage == kStages - 1 ? 0 : stage + 1;
+        float s[2][4];
+        {
+            // four chains of products instead of two: a chain's length is what a lone warp waits for
+            float s2[2][4];
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) s[n][x] = s2[n][x] = 0.f;
+#pragma unroll
+            for (int c = 0; c < kSets; ++c)
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const uint4 w = at[(8 * n + g) * kChunks + ((4 * c + t) ^ ((g & 1) << 2))];
+                    mma16816(s[n], qf[c][0], w.x, w.y);
+                    mma16816(s2[n], qf[c][1], w.z, w.w);
+                }
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) s[n][x] += s2[n][x];
+        }
         uint32_t pf[4] = {0u, 0u, 0u, 0u};
         float alpha[kRowsPerLane];
         bool moved = false;
@@ -173,8 +206,12 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kernel(const DecodeArgs 
         }
 #pragma unroll
         for (int e = 0; e < kHalves; ++e) {
-            const uint32_t w[4][4] = {{vf[e][0].x, vf[e][0].y, vf[e][0].z, vf[e][0].w}, {vf[e][1].x, vf[e][1].y, vf[e][1].z, vf[e][1].w},
-                                      {vf[e][2].x, vf[e][2].y, vf[e][2].z, vf[e][2].w}, {vf[e][3].x, vf[e][3].y, vf[e][3].z, vf[e][3].w}};
+            uint32_t w[4][4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint4 x = at[(kTile + 2 * t + (i & 1) + 8 * (i >> 1)) * kChunks + ((8 * e + g) ^ (t << 1))];
+                w[i][0] = x.x, w[i][1] = x.y, w[i][2] = x.z, w[i][3] = x.w;
+            }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
@@ -187,7 +224,9 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kernel(const DecodeArgs 
             }
         }
     }
-    // the warps of the CTA meet: every warp leaves its sums relative to its own maximum
+    // the warps of the CTA meet, over the stages: every warp leaves its sums relative to its own maximum
+    copy_wait<0>();
+    __syncthreads();
 #pragma unroll
     for (int x = 0; x < kRowsPerLane; ++x) {
         l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
@@ -228,37 +267,66 @@ __global__ void __launch_bounds__(kThreads) attn_decode_kernel(const DecodeArgs 
     }
 }
 
-// One CTA per (sequence, head): joins the splits that hold keys, in their order.
+// One CTA per (sequence, head): joins the splits that hold keys. The sums are added in an order that depends on their number only.
+constexpr int kJoinThreads = 256;
+constexpr int kMaxSplits = 256;
 template <int D>
-__global__ void __launch_bounds__(D / 2) attn_decode_join_kernel(const DecodeArgs a) {
+__global__ void __launch_bounds__(kJoinThreads) attn_decode_join_kernel(const DecodeArgs a) {
+    constexpr int kGroups = kJoinThreads / (D / 2);
+    __shared__ float s_f[kMaxSplits];
+    __shared__ float2 s_x[kGroups][D / 2];
+    __shared__ float s_red[2][kJoinThreads / 32];
     pdl_launch_dependents();
-    const int h = blockIdx.x, b = blockIdx.y, e = threadIdx.x * 2;
+    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     pdl_wait();
     const int len = length_of(a, b), chunk = chunk_of(len, a.splits), n = (len + chunk - 1) / chunk;
     const long long part = ((long long)b * a.H + h) * a.splits;
-    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + part;
-    float M = kNoKey;
-    for (int i = 0; i < n; ++i) M = fmaxf(M, ml[i].x);
-    float L = 0.f, x0 = 0.f, x1 = 0.f;
-    for (int i = 0; i < n; ++i) {
-        const float f = fast_exp2(ml[i].x - M);
-        const float2 x = *reinterpret_cast<const float2*>(a.part_o + (part + i) * D + e);
-        L += ml[i].y * f;
-        x0 = fmaf(x.x, f, x0), x1 = fmaf(x.y, f, x1);
+    // thread i weighs split i
+    const float2 ml = tid < n ? reinterpret_cast<const float2*>(a.part_ml)[part + tid] : make_float2(kNoKey, 0.f);
+    float M = ml.x;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    if (lane == 0) s_red[0][warp] = M;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kJoinThreads / 32; ++w) M = fmaxf(M, s_red[0][w]);
+    const float f = fast_exp2(ml.x - M);
+    s_f[tid] = f;
+    float L = ml.y * f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    if (lane == 0) s_red[1][warp] = L;
+    __syncthreads();
+    L = 0.f;
+#pragma unroll
+    for (int w = 0; w < kJoinThreads / 32; ++w) L += s_red[1][w];
+    const int grp = tid / (D / 2), e = tid % (D / 2);
+    float x0 = 0.f, x1 = 0.f;
+#pragma unroll 4
+    for (int i = grp; i < n; i += kGroups) {
+        const float2 x = *reinterpret_cast<const float2*>(a.part_o + (part + i) * D + 2 * e);
+        x0 = fmaf(x.x, s_f[i], x0), x1 = fmaf(x.y, s_f[i], x1);
     }
-    const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);
-    *reinterpret_cast<uint32_t*>(a.out + ((long long)b * a.H + h) * D + e) = pack_bf16x2(x0 * inv, x1 * inv);
-    if (e == 0) a.lse[(long long)b * a.H + h] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
+    s_x[grp][e] = make_float2(x0, x1);
+    __syncthreads();
+    if (grp == 0) {
+#pragma unroll
+        for (int i = 1; i < kGroups; ++i) x0 += s_x[i][e].x, x1 += s_x[i][e].y;
+        const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);
+        *reinterpret_cast<uint32_t*>(a.out + ((long long)b * a.H + h) * D + 2 * e) = pack_bf16x2(x0 * inv, x1 * inv);
+        if (e == 0) a.lse[(long long)b * a.H + h] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
+    }
 }
 
 template <int D, int R>
 cudaError_t launch(const DecodeArgs& a, cudaStream_t stream) {
-    constexpr int smem = kWarps * R * D * int(sizeof(float));
+    constexpr int stages = kWarps * kStages * kTile * D * 2 * 2, sums = kWarps * R * D * int(sizeof(float));
+    constexpr int smem = stages > sums ? stages : sums;
     cudaError_t e = cudaFuncSetAttribute(attn_decode_kernel<D, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    e = launch_pdl(attn_decode_kernel<D, R>, dim3(a.splits, a.Hkv * a.head_blocks, a.B), dim3(kThreads), smem, stream, a);
+    e = launch_pdl(attn_decode_kernel<D, R>, dim3(a.Hkv * a.head_blocks, a.splits, a.B), dim3(kThreads), smem, stream, a);
     if (e != cudaSuccess || a.splits == 1) return e;
-    return launch_pdl(attn_decode_join_kernel<D>, dim3(a.H, a.B), dim3(D / 2), 0, stream, a);
+    return launch_pdl(attn_decode_join_kernel<D>, dim3(a.H, a.B), dim3(kJoinThreads), 0, stream, a);
 }
 
 }  // namespace
@@ -266,11 +334,13 @@ cudaError_t launch(const DecodeArgs& a, cudaStream_t stream) {
 int decode_splits(int B, int T, int H, int Hkv) {
     const int G = H / Hkv, R = G <= 8 ? 8 : 16;
     const long long items = (long long)B * Hkv * ((G + R - 1) / R);
-    // enough CTAs for several rounds of the card (sequences differ in length), of at least two tiles per warp each
-    long long splits = (148 * 8 + items - 1) / items;
-    const long long most = (T + 2 * kMinChunk - 1) / (2 * kMinChunk);
+    // Six CTAs per SM, three rounds of the two that fit: sequences differ in length, and parts of one long sequence end together
+    // (measured, 1 / 1.5 / 2 / 3 / 8 rounds: 64 sequences up to 4096 keys 74 / 73 / 72 / 72 / 72 us, 8 of 8192 keys 59 / 50 / 53 / 49 / 51 us,
+    // one of 109,000 keys 75 / 78 / 77 / 80 / 82 us). A part has at least two steps.
+    long long splits = (148 * 6 + items - 1) / items;
+    const long long most = (T + 2 * kRound - 1) / (2 * kRound);
     if (splits > most) splits = most;
-    if (splits > 256) splits = 256;
+    if (splits > kMaxSplits) splits = kMaxSplits;
     return splits < 1 ? 1 : int(splits);
 }
 
