@@ -42,7 +42,7 @@ int b200loss_cross_entropy(const float* logits, const int* targets, float* d_log
  * Logits are rows of V elements of `dtype` (B200LOSS_F32 or B200LOSS_BF16), row i at logits + i * row_stride elements, at
  * any alignment that fits the type; outputs are FP32 (int32 for tokens), sums are held in FP32. A logit of -inf is a token
  * that is not allowed (p = 0); in a row that allows none every log-probability is -inf and the entropy 0. A row with a NaN
- * or +inf gives NaN (a NaN ranks above every number among the alternatives). 0 < temperature < inf. rows = 0 is a no-op.
+ * or +inf gives NaN (a NaN ranks above every number among the alternatives). 1e-6 <= temperature <= 1e6. rows = 0 is a no-op.
  * Allocates nothing and holds no state: calls may overlap and be captured. No counterpart in the reference. */
 int b200loss_token_logprobs(const void* logits, int dtype, long long row_stride, const int* targets, int rows, int V,
                             float temperature, float* logprobs, float* entropy, float* stats, int top, float* top_logprobs,

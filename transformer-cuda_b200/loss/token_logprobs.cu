@@ -10,10 +10,11 @@
 // them the exponential, which leaves the SM half idle at the rate BF16 logits arrive.
 //
 // Top alternatives cost nothing per logit: the maximum that every thread keeps for the softmax anyway gives a threshold (the
-// k-th largest of the thread maxima) that at least k logits reach, and only the threads whose maximum reaches it can own an
-// alternative. Their logits, about k / threads of the row, are read again (from L2), the few that reach the threshold are
-// ranked by counting. Order: larger logit first, equal ones by the lower index. A row with more candidates than the list holds
-// (many equal logits, or fewer allowed tokens than alternatives) falls back to one pass per alternative.
+// k-th largest of the thread maxima, or a little less) that at least k logits reach. A thread also leaves the maximum of each
+// eighth of its logits; only those that reach the threshold are read again, a percent of a long row, and the few logits that reach
+// it are ranked by counting. (Reading all logits of such threads again cost as much as a fifth of the row: 20 alternatives of
+// 4096 x 131072 BF16 logits 57 us on top of 166.) Order: larger logit first, equal ones by the lower index. A row with more
+// candidates than the lists hold (many equal logits, or fewer allowed tokens than alternatives) falls back to one pass per alternative.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -27,15 +28,33 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
+constexpr int kWarpRowThreads = 256; // CTAs of the kernels that give a row to a warp
 constexpr int kUnroll = 4;           // 16-byte loads in flight per thread
 constexpr int kMaxTop = 32;
 constexpr int kMaxCand = 1024;
+constexpr int kSegments = 8;
+constexpr int kMaxHot = 256;
 constexpr int kMaxCluster = 8;
 constexpr int kWarpRowVocab = 1024;  // rows up to here are handled by one warp each
+constexpr int kWarpGradVocab = 256;  // the same in the gradient
+constexpr int kSmallRowVecs = 1024;  // rows of up to so many 16-byte vectors by CTAs of 64 threads, longer ones by 256
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -1e30f;    // x - m is held above this, so that a masked logit contributes 0 * finite
+constexpr float kFloor = -0x1.92p99f; // -9.95e29, a BF16 value: logits enter the sums of a row as at least this (see Stat)
+constexpr float kWild = 1e29f;       // maxima beyond this take the exact pass
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Maximum that a NaN passes through: a row that holds one ends as NaN instead of losing it.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
 
 // ---------------------------------------------------------------- element access
 template <typename T>
@@ -48,6 +67,22 @@ struct Elem<float> {
     static __device__ __forceinline__ void store(float* p, float x) { *p = x; }
     static __device__ __forceinline__ void unpack(const uint4& w, float* x) {
         x[0] = __uint_as_float(w.x), x[1] = __uint_as_float(w.y), x[2] = __uint_as_float(w.z), x[3] = __uint_as_float(w.w);
+    }
+    static __device__ __forceinline__ uint4 raise(uint4 w) {  // every element to at least kFloor
+        w.x = max1(w.x), w.y = max1(w.y), w.z = max1(w.z), w.w = max1(w.w);
+        return w;
+    }
+    static __device__ __forceinline__ uint32_t max1(uint32_t x) { return __float_as_uint(max_nan(__uint_as_float(x), kFloor)); }
+    template <int N>
+    static __device__ __forceinline__ float largest(const uint4 (&w)[N]) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            float x[4];
+            unpack(w[u], x);
+            m = max_nan(max_nan(m, max_nan(x[0], x[1])), max_nan(x[2], x[3]));
+        }
+        return m;
     }
     static __device__ __forceinline__ uint4 pack(const float* x) {
         return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
@@ -66,6 +101,24 @@ struct Elem<__nv_bfloat16> {
             x[2 * i] = __uint_as_float(u[i] << 16);
             x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
         }
+    }
+    // packed pairs: half the instructions of single maxima
+    static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+        uint32_t y;
+        asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(y) : "r"(a), "r"(b));
+        return y;
+    }
+    static __device__ __forceinline__ uint4 raise(uint4 w) {
+        constexpr uint32_t floor2 = 0xf149f149u;  // kFloor, twice
+        w.x = max2(w.x, floor2), w.y = max2(w.y, floor2), w.z = max2(w.z, floor2), w.w = max2(w.w, floor2);
+        return w;
+    }
+    template <int N>
+    static __device__ __forceinline__ float largest(const uint4 (&w)[N]) {
+        uint32_t m = kNegInf;
+#pragma unroll
+        for (int u = 0; u < N; ++u) m = max2(max2(m, max2(w[u].x, w[u].y)), max2(w[u].z, w[u].w));
+        return max_nan(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
     }
     static __device__ __forceinline__ uint4 pack(const float* x) {
         uint32_t u[4];
@@ -93,17 +146,6 @@ __device__ __forceinline__ RowSplit split_row(const T* row, int V) {
 }
 
 // ---------------------------------------------------------------- arithmetic
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-// Maximum that a NaN passes through: a row that holds one ends as NaN instead of losing it.
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float y;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
-    return y;
-}
 // Packed pairs of FP32: one instruction for two operations.
 struct Pair {
     uint64_t v;
@@ -130,18 +172,18 @@ __device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
     return r;
 }
 
-// m, s and t of a part of a row. Nothing seen yet, or only masked logits: m = -inf, s = t = 0.
+// A part of a row: its maximum m, s = sum 2^a and t = sum a 2^a with a = c (x - m), c = log2(e) / temperature.
+// Logits enter the sums as at least kFloor, which costs one packed maximum and keeps every a and every m finite (a masked logit
+// adds 0 * finite, not 0 * inf). That changes nothing unless the row's maximum is below kFloor / 10 or so itself: rows with a
+// maximum outside +-kWild (a row of masked logits, of the type's lowest value, of NaN or +inf) are summed again without it.
 struct Stat {
     float m, s, t;
 };
-// `a` with its sums taken relative to the larger maximum M (c = log2(e) / temperature).
+// `a` with its sums taken relative to the larger maximum M.
 __device__ __forceinline__ void rebase(Stat& a, float M, float c) {
-    if (a.m == M) return;
-    if (a.m != -INFINITY) {
-        const float d = a.m - M, f = ex2(fmaxf(d, kLowest) * c);
-        a.t = (a.t + a.s * fmaxf(d, kLowest)) * f;
-        a.s *= f;
-    }
+    const float d = fmaxf((a.m - M) * c, -1000.f), f = ex2(d);  // 2^-1000 is 0, and s d stays finite
+    a.t = fmaf(a.s, d, a.t) * f;
+    a.s *= f;
     a.m = M;
 }
 __device__ __forceinline__ Stat merge(Stat a, Stat b, float c) {
@@ -150,16 +192,30 @@ __device__ __forceinline__ Stat merge(Stat a, Stat b, float c) {
     rebase(b, M, c);
     return Stat{M, a.s + b.s, a.t + b.t};
 }
-__device__ __forceinline__ Stat shuffle_merge(Stat a, float c) {
+// What the outputs need of a whole row.
+struct RowStat {
+    float m, ln_s, entropy;  // ln_s: of the sum relative to m
+};
+__device__ __forceinline__ RowStat finish(const Stat& a) {
+    if (a.m == -INFINITY) return RowStat{a.m, 0.f, 0.f};  // no token is allowed
+    const float log2_s = log2f(a.s);
+    return RowStat{a.m, log2_s * kLn2, (log2_s - a.t / a.s) * kLn2};
+}
+// s and t of a row (or of a part of it) whose maximum m is known, in exact steps and with every logit as it is: one element.
+__device__ __forceinline__ void add_exact(float x, float m, float c, float& s, float& t) {
+    const float a = max_nan(x - m, kLowest) * c, e = ex2(a);
+    s += e;
+    t = fmaf(e, a, t);
+}
+__device__ __forceinline__ float warp_add(float x) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        Stat b;
-        b.m = __shfl_xor_sync(0xffffffffu, a.m, o);
-        b.s = __shfl_xor_sync(0xffffffffu, a.s, o);
-        b.t = __shfl_xor_sync(0xffffffffu, a.t, o);
-        a = merge(a, b, c);
-    }
-    return a;
+    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+    return x;
+}
+__device__ __forceinline__ float warp_max_nan(float x) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) x = max_nan(x, __shfl_xor_sync(0xffffffffu, x, o));
+    return x;
 }
 
 // Whole numbers in the order of the logits (-0 = +0; NaN above every number, below the all-ones bound of a search), and back.
@@ -191,31 +247,53 @@ struct FwdArgs {
 };
 
 // A row without an allowed token (every logit -inf): every log-probability is -inf, the entropy 0.
-__device__ __forceinline__ float logprob_of(float x, const Stat& a, float ln_s, float inv_temperature) {
-    return a.m == -INFINITY ? -INFINITY : (x - a.m) * inv_temperature - ln_s;
+__device__ __forceinline__ float logprob_of(float x, const RowStat& a, float inv_temperature) {
+    return a.m == -INFINITY ? -INFINITY : fmaf(x - a.m, inv_temperature, -a.ln_s);
 }
 template <typename T>
-__device__ __forceinline__ float write_row(const FwdArgs& a, const T* row, int r, const Stat& st) {
-    const float ln_s = st.m == -INFINITY ? 0.f : logf(st.s);
+__device__ __forceinline__ void write_row(const FwdArgs& a, const T* row, int r, const RowStat& st) {
     const int target = a.targets[r];
     a.stats[2ll * r] = st.m;
-    a.stats[2ll * r + 1] = ln_s;
-    a.entropy[r] = st.m == -INFINITY ? 0.f : ln_s - a.inv_temperature * (st.t / st.s);
-    a.logprobs[r] = (unsigned)target < (unsigned)a.V ? logprob_of(Elem<T>::load(row + target), st, ln_s, a.inv_temperature) : 0.f;
-    return ln_s;
+    a.stats[2ll * r + 1] = st.ln_s;
+    a.entropy[r] = st.entropy;
+    a.logprobs[r] = (unsigned)target < (unsigned)a.V ? logprob_of(Elem<T>::load(row + target), st, a.inv_temperature) : 0.f;
 }
 
 // ---------------------------------------------------------------- forward, one CTA (or one cluster of CTAs) per row
-template <typename T>
+// A threshold that at least `top` (<= 32) and hardly more of the warp's 32 N keys reach: bisection between the smallest of the 32
+// lane maxima (which 32 keys reach) and the largest key. Executed by one warp.
+template <int N>
+__device__ __forceinline__ uint32_t threshold_of(const uint32_t (&k)[N], int top) {
+    uint32_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) mine = max(mine, k[i]);
+    uint32_t lo = __reduce_min_sync(0xffffffffu, mine), hi = __reduce_max_sync(0xffffffffu, mine) + 1u;
+    while (hi - lo > 1u) {
+        const uint32_t mid = lo + (hi - lo) / 2u;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) n += __popc(__ballot_sync(0xffffffffu, k[i] >= mid));
+        if (n < top) {
+            hi = mid;
+        } else {
+            lo = mid;
+            if (n <= top + 4) break;
+        }
+    }
+    return lo;
+}
+
+template <typename T, int kThreads>
 __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const FwdArgs a) {
-    constexpr int E = Elem<T>::kPerVec;
-    __shared__ Stat s_stat[kWarps];
-    __shared__ Stat s_row;
+    constexpr int E = Elem<T>::kPerVec, kWarps = kThreads / 32;
+    __shared__ float s_max[kWarps], s_sum[kWarps], s_sum_a[kWarps], s_part_max;
+    __shared__ Stat s_part, s_total;  // of this CTA's part of the row, and of the row
     __shared__ uint32_t s_key[kThreads];
     __shared__ uint64_t s_cand[kMaxCand];
     __shared__ uint64_t s_sel[kMaxTop];
     __shared__ uint64_t s_best[kWarps];
-    __shared__ int s_hot[kThreads];
+    __shared__ float s_segment[kSegments][kThreads];
+    __shared__ int s_hot[kMaxHot];  // segments that hold a candidate: thread + kThreads * segment
     __shared__ int s_nhot, s_ncand;
     __shared__ uint32_t s_threshold;
 
@@ -233,94 +311,109 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const FwdArgs 
     const int edge = (part == 0 && tid < sp.head) ? tid
                      : (part == parts - 1 && tid >= 32 && tid < 32 + sp.tail) ? sp.head + sp.vecs * E + (tid - 32)
                                                                               : -1;
-    Stat st{-INFINITY, 0.f, 0.f};
+    Stat st{kFloor, 0.f, 0.f};
+    float my_max = -INFINITY;  // of the logits as they are: what the alternatives are found by, and whether the row is wild
     if (edge >= 0) {
-        st.m = Elem<T>::load(row + edge);
-        st.s = st.m == -INFINITY ? 0.f : (st.m - st.m) + 1.f;  // +inf and NaN make NaN here
+        my_max = Elem<T>::load(row + edge);
+        st.m = max_nan(my_max, kFloor);
+        st.s = 1.f;
     }
     Pair s2 = pair(st.s, 0.f), t2 = pair(0.f, 0.f);
-    for (int i0 = begin; i0 < end; i0 += kThreads * kUnroll) {
-        uint4 w[kUnroll];
+    const Pair c2 = pair(c, c);
+    const uint4 nothing = make_uint4(Elem<T>::kNegInf, Elem<T>::kNegInf, Elem<T>::kNegInf, Elem<T>::kNegInf);
+    uint4 next[kUnroll];  // the next round's loads are under way while this one is added
+    auto load_round = [&](int i0) {
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
             const int i = i0 + u * kThreads + tid;
-            w[u] = i < end ? __ldg(vec + i) : make_uint4(Elem<T>::kNegInf, Elem<T>::kNegInf, Elem<T>::kNegInf, Elem<T>::kNegInf);
+            next[u] = i < end ? __ldg(vec + i) : nothing;
         }
-        float mx = st.m;
+    };
+    load_round(begin);
+    // The row's rounds in at most kSegments segments: a thread's maximum is kept for each (alternatives only).
+    const int rounds = (end - begin + kThreads * kUnroll - 1) / (kThreads * kUnroll), per_segment = max(1, (rounds + kSegments - 1) / kSegments);
+    float segment_max = -INFINITY;
+    int segment = 0, left = per_segment;
+    for (int i0 = begin; i0 < end; i0 += kThreads * kUnroll) {
+        uint4 w[kUnroll];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            float x[E];
-            Elem<T>::unpack(w[u], x);
-#pragma unroll
-            for (int e = 0; e < E; ++e) mx = max_nan(mx, x[e]);
+        for (int u = 0; u < kUnroll; ++u) w[u] = next[u];
+        if (i0 + kThreads * kUnroll < end) load_round(i0 + kThreads * kUnroll);
+        const float round_max = Elem<T>::largest(w);
+        my_max = max_nan(my_max, round_max);
+        if (a.top > 0) {
+            segment_max = max_nan(segment_max, round_max);
+            if (--left == 0 || i0 + kThreads * kUnroll >= end) {
+                s_segment[segment++][tid] = segment_max;
+                segment_max = -INFINITY, left = per_segment;
+            }
         }
-        if (mx != st.m) {  // a new maximum, or NaN
+        const float m = max_nan(st.m, my_max);
+        if (m != st.m) {  // a new maximum, or NaN
             float sa, sb, ta, tb;
             split(s2, sa, sb), split(t2, ta, tb);
             Stat old{st.m, sa + sb, ta + tb};
-            rebase(old, mx, c);
-            st.m = mx;
+            rebase(old, m, c);
+            st.m = m;
             s2 = pair(old.s, 0.f), t2 = pair(old.t, 0.f);
         }
-        if (st.m == -INFINITY) continue;
-        const Pair neg_m = pair(-st.m, -st.m), c2 = pair(c, c);
+        const Pair neg_m = pair(-st.m, -st.m);
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
+            if (i0 + u * kThreads + warp * 32 >= end) break;  // the last round's rest: nothing for this warp
             float x[E];
-            Elem<T>::unpack(w[u], x);
+            Elem<T>::unpack(Elem<T>::raise(w[u]), x);
 #pragma unroll
             for (int e = 0; e < E; e += 2) {
-                float d0, d1, a0, a1;
-                split(add(pair(x[e], x[e + 1]), neg_m), d0, d1);
-                const Pair d = pair(max_nan(d0, kLowest), max_nan(d1, kLowest));
-                split(mul(d, c2), a0, a1);
+                float a0, a1;
+                const Pair arg = mul(add(pair(x[e], x[e + 1]), neg_m), c2);
+                split(arg, a0, a1);
                 const Pair ex = pair(ex2(a0), ex2(a1));
                 s2 = add(s2, ex);
-                t2 = fma(ex, d, t2);
+                t2 = fma(ex, arg, t2);
             }
         }
     }
-    const float my_max = st.m;
     {
         float sa, sb, ta, tb;
         split(s2, sa, sb), split(t2, ta, tb);
         st.s = sa + sb, st.t = ta + tb;
     }
-    st = shuffle_merge(st, c);
-    if (lane == 0) s_stat[warp] = st;
+    const float warp_max = warp_max_nan(my_max);
+    if (lane == 0) s_max[warp] = warp_max;
     s_key[tid] = to_key(my_max);
     if (tid == 0) s_nhot = 0, s_ncand = 0;
     __syncthreads();
-    if (warp == 0) {
-        Stat x = lane < kWarps ? s_stat[lane] : Stat{-INFINITY, 0.f, 0.f};
-        x = shuffle_merge(x, c);
-        if (lane == 0) s_row = x;
-        if (a.top > 0) {  // k-th largest thread maximum
-            uint32_t k[kThreads / 32], best = 0;
+    float part_max = s_max[0];
 #pragma unroll
-            for (int i = 0; i < kThreads / 32; ++i) k[i] = s_key[i * 32 + lane];
-            for (int n = 0; n < a.top; ++n) {
-                uint32_t mine = 0;
+    for (int w = 1; w < kWarps; ++w) part_max = max_nan(part_max, s_max[w]);
+    rebase(st, max_nan(part_max, kFloor), c);
+    const float warp_s = warp_add(st.s), warp_t = warp_add(st.t);
+    if (lane == 0) s_sum[warp] = warp_s, s_sum_a[warp] = warp_t;
+    if (a.top > 0 && warp == kWarps - 1) {
+        uint32_t k[kWarps];
 #pragma unroll
-                for (int i = 0; i < kThreads / 32; ++i) mine = max(mine, k[i]);
-                best = __reduce_max_sync(0xffffffffu, mine);
-                const uint32_t who = __ballot_sync(0xffffffffu, mine == best);
-                if (lane == __ffs(who) - 1) {
-                    bool gone = false;
-#pragma unroll
-                    for (int i = 0; i < kThreads / 32; ++i)
-                        if (!gone && k[i] == best) k[i] = 0, gone = true;
-                }
-            }
-            if (lane == 0) s_threshold = best;
-        }
+        for (int i = 0; i < kWarps; ++i) k[i] = s_key[i * 32 + lane];
+        const uint32_t threshold = threshold_of(k, a.top);
+        if (lane == 0) s_threshold = threshold;
     }
     __syncthreads();
+    if (tid == 0) {
+        Stat x{max_nan(part_max, kFloor), 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) x.s += s_sum[w], x.t += s_sum_a[w];
+        s_part = x, s_part_max = part_max;
+    }
 
     if (a.top > 0) {
         // a masked logit is only ever an alternative where fewer tokens are allowed than alternatives asked for: the fallback
         const uint32_t threshold = max(s_threshold, kKeyNegInf + 1u);
-        if (s_key[tid] >= threshold) s_hot[atomicAdd(&s_nhot, 1)] = tid;
+        if (s_key[tid] >= threshold)
+            for (int i = 0; i < segment; ++i)  // its own: no other thread has written them
+                if (to_key(s_segment[i][tid]) >= threshold) {
+                    const int at = atomicAdd(&s_nhot, 1);
+                    if (at < kMaxHot) s_hot[at] = tid + kThreads * i;
+                }
         __syncthreads();
         const int nhot = s_nhot;
         auto consider = [&](float x, int index) {
@@ -329,19 +422,35 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const FwdArgs 
             const int at = atomicAdd(&s_ncand, 1);
             if (at < kMaxCand) s_cand[at] = candidate(key, index);
         };
-        for (int h = warp; h < nhot; h += kWarps) {
-            const int owner = s_hot[h];
-            for (int i = begin + owner + lane * kThreads; i < end; i += 32 * kThreads) {
-                float x[E];
-                Elem<T>::unpack(__ldg(vec + i), x);
+        // every (segment, vector of it) to a thread of its own, several at a time, so that the reads are under way together
+        const int per = per_segment * kUnroll, pairs = nhot <= kMaxHot ? nhot * per : 0;
+        for (int i0 = tid; i0 < pairs; i0 += kThreads * kUnroll) {
+            uint4 w[kUnroll];
+            int at[kUnroll];
 #pragma unroll
-                for (int e = 0; e < E; ++e) consider(x[e], sp.head + i * E + e);
+            for (int u = 0; u < kUnroll; ++u) {
+                const int i = i0 + u * kThreads;
+                at[u] = end;
+                if (i < pairs) {
+                    const int hot = s_hot[i / per];
+                    at[u] = begin + hot % kThreads + ((hot / kThreads) * per + i % per) * kThreads;
+                }
+                w[u] = at[u] < end ? __ldg(vec + at[u]) : nothing;
+            }
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                const uint4 one[1] = {w[u]};
+                if (to_key(Elem<T>::largest(one)) < threshold) continue;
+                float x[E];
+                Elem<T>::unpack(w[u], x);
+#pragma unroll
+                for (int e = 0; e < E; ++e) consider(x[e], sp.head + at[u] * E + e);
             }
         }
         if (edge >= 0) consider(Elem<T>::load(row + edge), edge);
         __syncthreads();
         const int n = s_ncand;
-        if (n >= a.top && n <= kMaxCand) {
+        if (n >= a.top && n <= kMaxCand && nhot <= kMaxHot) {
             for (int i = tid; i < n; i += kThreads) {
                 const uint64_t mine = s_cand[i];
                 int rank = 0;
@@ -381,13 +490,43 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const FwdArgs 
         }
     }
 
+    // the row's maximum, and whether it has to be summed again (every CTA of the row comes to the same answer)
+    float row_max = part_max;
+    if (parts > 1) {
+        cluster.sync();
+        for (int p = 0; p < parts; ++p) row_max = max_nan(row_max, *cluster.map_shared_rank(&s_part_max, p));
+    }
+    const bool wild = !(fabsf(row_max) < kWild);
+    if (wild) {
+        float s = 0.f, t = 0.f;
+        if (row_max != -INFINITY) {
+            for (int i = begin + tid; i < end; i += kThreads) {
+                float x[E];
+                Elem<T>::unpack(__ldg(vec + i), x);
+#pragma unroll
+                for (int e = 0; e < E; ++e) add_exact(x[e], row_max, c, s, t);
+            }
+            if (edge >= 0) add_exact(Elem<T>::load(row + edge), row_max, c, s, t);
+        }
+        s = warp_add(s), t = warp_add(t);
+        __syncthreads();  // s_sum has been read
+        if (lane == 0) s_sum[warp] = s, s_sum_a[warp] = t;
+        __syncthreads();
+        if (tid == 0) {
+            for (int w = 1; w < kWarps; ++w) s += s_sum[w], t += s_sum_a[w];
+            s_part = Stat{row_max, s, t};
+        }
+    }
     if (parts > 1) {  // rank 0 joins what the CTAs of the row found
         cluster.sync();
         if (part == 0) {
             if (tid == 0) {
-                Stat x = s_row;
-                for (int p = 1; p < parts; ++p) x = merge(x, *cluster.map_shared_rank(&s_row, p), c);
-                s_stat[0] = x;
+                Stat x = s_part;
+                for (int p = 1; p < parts; ++p) {
+                    const Stat y = *cluster.map_shared_rank(&s_part, p);
+                    x = wild ? Stat{row_max, x.s + y.s, x.t + y.t} : merge(x, y, c);
+                }
+                s_total = x;
             }
             const int n = parts * a.top;
             for (int i = tid; i < n; i += kThreads) s_cand[i] = cluster.map_shared_rank(s_sel, i / a.top)[i % a.top];
@@ -401,48 +540,71 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const FwdArgs 
             for (int j = 0; j < n; ++j) rank += s_cand[j] > mine;
             if (mine != 0 && rank < a.top) s_sel[rank] = mine;
         }
-        if (tid == 0) s_row = s_stat[0];
+    } else if (tid == 0) {
+        s_total = s_part;
     }
     __syncthreads();
-    const Stat total = s_row;
+    const RowStat total = finish(s_total);
     if (tid == 0) write_row(a, row, r, total);
     if (tid < a.top) {
-        const float ln_s = total.m == -INFINITY ? 0.f : logf(total.s);
         const uint64_t y = s_sel[tid];
-        a.top_logprobs[(long long)r * a.top + tid] = logprob_of(from_key(uint32_t(y >> 32)), total, ln_s, a.inv_temperature);
+        a.top_logprobs[(long long)r * a.top + tid] = logprob_of(from_key(uint32_t(y >> 32)), total, a.inv_temperature);
         a.top_tokens[(long long)r * a.top + tid] = index_of(y);
     }
 }
 
 // ---------------------------------------------------------------- forward, one warp per (short) row
 template <typename T>
-__global__ void __launch_bounds__(kThreads) token_logprobs_warp_kernel(const FwdArgs a) {
-    const int lane = threadIdx.x & 31;
-    const long long r64 = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
+__global__ void __launch_bounds__(kWarpRowThreads) token_logprobs_warp_kernel(const FwdArgs a) {
+    constexpr int kWarps = kWarpRowThreads / 32, kList = 128;
+    __shared__ uint64_t s_cand[kWarps][kList];
+    __shared__ int s_ncand[kWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const long long r64 = (long long)blockIdx.x * kWarps + warp;
     if (r64 >= a.rows) return;
     const int r = int(r64);
     const T* row = static_cast<const T*>(a.logits) + a.row_stride * r;
     const float c = a.inv_temperature * kLog2e;
-    Stat st{-INFINITY, 0.f, 0.f};
-    for (int v = lane; v < a.V; v += 32) st.m = max_nan(st.m, Elem<T>::load(row + v));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) st.m = max_nan(st.m, __shfl_xor_sync(0xffffffffu, st.m, o));
+    float mine = -INFINITY;
+    for (int v = lane; v < a.V; v += 32) mine = max_nan(mine, Elem<T>::load(row + v));
+    Stat st{warp_max_nan(mine), 0.f, 0.f};
     if (st.m != -INFINITY) {
-        for (int v = lane; v < a.V; v += 32) {
-            const float d = max_nan(Elem<T>::load(row + v) - st.m, kLowest), e = ex2(d * c);
-            st.s += e;
-            st.t = fmaf(e, d, st.t);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            st.s += __shfl_xor_sync(0xffffffffu, st.s, o);
-            st.t += __shfl_xor_sync(0xffffffffu, st.t, o);
+        for (int v = lane; v < a.V; v += 32) add_exact(Elem<T>::load(row + v), st.m, c, st.s, st.t);
+        st.s = warp_add(st.s), st.t = warp_add(st.t);
+    }
+    const RowStat total = finish(st);
+    if (lane == 0) write_row(a, row, r, total);
+    if (a.top == 0) return;
+
+    // alternatives: as above, with the lane maxima; rows too short for 32 lanes have threshold 0 (every logit is a candidate)
+    const uint32_t k[1] = {lane < a.V ? to_key(mine) : 0u};
+    const uint32_t threshold = threshold_of(k, a.top);
+    if (lane == 0) s_ncand[warp] = 0;
+    __syncwarp();
+    for (int v = lane; v < a.V; v += 32) {
+        const uint32_t key = to_key(Elem<T>::load(row + v));
+        if (key >= threshold) {
+            const int at = atomicAdd(&s_ncand[warp], 1);
+            if (at < kList) s_cand[warp][at] = candidate(key, v);
         }
     }
-    if (lane == 0) write_row(a, row, r, st);
-    const float ln_s = st.m == -INFINITY ? 0.f : logf(st.s);
+    __syncwarp();
+    const int n = s_ncand[warp];
+    auto write = [&](int rank, uint64_t y) {
+        a.top_logprobs[(long long)r * a.top + rank] = logprob_of(from_key(uint32_t(y >> 32)), total, a.inv_temperature);
+        a.top_tokens[(long long)r * a.top + rank] = index_of(y);
+    };
+    if (n <= kList) {
+        for (int i = lane; i < n; i += 32) {
+            const uint64_t y = s_cand[warp][i];
+            int rank = 0;
+            for (int j = 0; j < n; ++j) rank += s_cand[warp][j] > y;
+            if (rank < a.top) write(rank, y);
+        }
+        return;
+    }
     uint64_t before = ~uint64_t(0);
-    for (int k = 0; k < a.top; ++k) {
+    for (int i = 0; i < a.top; ++i) {
         uint64_t best = 0;
         for (int v = lane; v < a.V; v += 32) {
             const uint64_t y = candidate(to_key(Elem<T>::load(row + v)), v);
@@ -453,10 +615,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_warp_kernel(const Fwd
             const uint64_t y = __shfl_xor_sync(0xffffffffu, best, o);
             if (y > best) best = y;
         }
-        if (lane == 0) {
-            a.top_logprobs[(long long)r * a.top + k] = logprob_of(from_key(uint32_t(best >> 32)), st, ln_s, a.inv_temperature);
-            a.top_tokens[(long long)r * a.top + k] = index_of(best);
-        }
+        if (lane == 0) write(i, best);
         before = best;
     }
 }
@@ -495,13 +654,13 @@ __device__ __forceinline__ RowGrad row_grad(const BwdArgs& p, int r) {
     q.b = -p.inv_temperature * p.inv_temperature * ge;
     return q;
 }
-__device__ __forceinline__ float grad_of(const RowGrad& q, float x, float c, int v) {
+__device__ __forceinline__ float grad_of(const RowGrad& q, float x, float c) {  // without the target's own term
     const float d = max_nan(x - q.m, kLowest);
-    return fmaf(ex2(fmaf(d, c, -q.l)), fmaf(d, q.b, q.a), v == q.target ? q.g : 0.f);
+    return ex2(fmaf(d, c, -q.l)) * fmaf(d, q.b, q.a);
 }
 
 // One CTA per row and chunk of vectors; logits and dlogits are at the same distance from a 16-byte boundary in every row.
-template <typename T>
+template <typename T, int kThreads>
 __global__ void __launch_bounds__(kThreads) token_logprobs_bwd_kernel(const BwdArgs a) {
     constexpr int E = Elem<T>::kPerVec;
     const int r = int(blockIdx.x / unsigned(a.chunks)), chunk = int(blockIdx.x % unsigned(a.chunks));
@@ -534,7 +693,13 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_bwd_kernel(const BwdA
                 float x[E];
                 Elem<T>::unpack(w[u], x);
 #pragma unroll
-                for (int e = 0; e < E; ++e) x[e] = grad_of(q, x[e], c, sp.head + i * E + e);
+                for (int e = 0; e < E; ++e) x[e] = grad_of(q, x[e], c);
+                const int at = q.target - (sp.head + i * E);
+                if ((unsigned)at < (unsigned)E) {
+#pragma unroll
+                    for (int e = 0; e < E; ++e)
+                        if (e == at) x[e] += q.g;
+                }
                 dst[i] = Elem<T>::pack(x);
             }
         }
@@ -543,12 +708,13 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_bwd_kernel(const BwdA
     const int edge = (chunk == 0 && tid < sp.head) ? tid
                      : (chunk == a.chunks - 1 && tid >= 32 && tid < 32 + sp.tail) ? sp.head + sp.vecs * E + (tid - 32)
                                                                                   : -1;
-    if (edge >= 0) Elem<T>::store(out + edge, q.zero ? 0.f : grad_of(q, Elem<T>::load(row + edge), c, edge));
+    if (edge >= 0) Elem<T>::store(out + edge, q.zero ? 0.f : grad_of(q, Elem<T>::load(row + edge), c) + (edge == q.target ? q.g : 0.f));
 }
 
 // One warp per row: short rows, and rows of dlogits at another distance from a 16-byte boundary than the logits'.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) token_logprobs_bwd_warp_kernel(const BwdArgs a) {
+__global__ void __launch_bounds__(kWarpRowThreads) token_logprobs_bwd_warp_kernel(const BwdArgs a) {
+    constexpr int kWarps = kWarpRowThreads / 32;
     const int lane = threadIdx.x & 31;
     const long long r64 = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
     if (r64 >= a.rows) return;
@@ -557,7 +723,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_bwd_warp_kernel(const
     T* out = static_cast<T*>(a.dlogits) + a.d_row_stride * r;
     const RowGrad q = row_grad(a, r);
     const float c = a.inv_temperature * kLog2e;
-    for (int v = lane; v < a.V; v += 32) Elem<T>::store(out + v, q.zero ? 0.f : grad_of(q, Elem<T>::load(row + v), c, v));
+    for (int v = lane; v < a.V; v += 32) Elem<T>::store(out + v, q.zero ? 0.f : grad_of(q, Elem<T>::load(row + v), c) + (v == q.target ? q.g : 0.f));
 }
 
 // ---------------------------------------------------------------- host side
@@ -575,19 +741,14 @@ int check_common(const char* null_text, bool any_null, int dtype, int rows, int 
     if (dtype != B200LOSS_F32 && dtype != B200LOSS_BF16) return fail(B200LOSS_ERR_ARG, "token_logprobs: dtype must be B200LOSS_F32 or B200LOSS_BF16");
     if (rows < 0 || V <= 0) return fail(B200LOSS_ERR_ARG, "token_logprobs: rows must not be negative and V must be positive");
     if (row_stride < V) return fail(B200LOSS_ERR_ARG, "token_logprobs: row_stride is smaller than V");
-    if (!(temperature > 0.f) || !isfinite(temperature) || !isfinite(1.0f / temperature))
-        return fail(B200LOSS_ERR_ARG, "token_logprobs: temperature must be positive and finite");
+    if (!(temperature >= 1e-6f && temperature <= 1e6f)) return fail(B200LOSS_ERR_ARG, "token_logprobs: temperature must be between 1e-6 and 1e6");
     if (rows > 0 && any_null) return fail(B200LOSS_ERR_ARG, null_text);
     return B200LOSS_OK;
 }
 bool misaligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) != 0; }
 
-template <typename T>
-cudaError_t launch_forward(const FwdArgs& a, cudaStream_t stream) {
-    if (a.V <= kWarpRowVocab) {
-        token_logprobs_warp_kernel<T><<<(a.rows + kWarps - 1) / kWarps, kThreads, 0, stream>>>(a);
-        return cudaGetLastError();
-    }
+template <typename T, int kThreads>
+cudaError_t launch_rows(const FwdArgs& a, cudaStream_t stream) {
     // Few rows: a cluster of CTAs shares one, so that the row is not read at the speed of one SM. Each CTA keeps at least one
     // full round of loads.
     int parts = 1;
@@ -603,22 +764,39 @@ cudaError_t launch_forward(const FwdArgs& a, cudaStream_t stream) {
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T>, a);
+    return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, kThreads>, a);
 }
 
 template <typename T>
-cudaError_t launch_backward(BwdArgs a, cudaStream_t stream) {
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a.logits), d = reinterpret_cast<uintptr_t>(a.dlogits);
-    const bool same_phase = ((x ^ d) & 15u) == 0 && ((a.row_stride - a.d_row_stride) * (long long)sizeof(T)) % 16 == 0;
-    if (a.V <= kWarpRowVocab || !same_phase) {
-        token_logprobs_bwd_warp_kernel<T><<<(a.rows + kWarps - 1) / kWarps, kThreads, 0, stream>>>(a);
+cudaError_t launch_forward(const FwdArgs& a, cudaStream_t stream) {
+    if (a.V <= kWarpRowVocab) {
+        constexpr int rows = kWarpRowThreads / 32;
+        token_logprobs_warp_kernel<T><<<(a.rows + rows - 1) / rows, kWarpRowThreads, 0, stream>>>(a);
         return cudaGetLastError();
     }
+    // a thread should have some vectors of its row: short rows get small CTAs
+    return a.V <= kSmallRowVecs * Elem<T>::kPerVec ? launch_rows<T, 64>(a, stream) : launch_rows<T, 256>(a, stream);
+}
+
+template <typename T, int kThreads>
+cudaError_t launch_gradient(BwdArgs a, cudaStream_t stream) {
     constexpr int per_cta = kThreads * kUnroll * Elem<T>::kPerVec;
     a.chunks = (a.V + per_cta - 1) / per_cta;
     if ((long long)a.rows * a.chunks > 0x7fffffffLL) return cudaErrorInvalidValue;
-    token_logprobs_bwd_kernel<T><<<unsigned(a.rows) * unsigned(a.chunks), kThreads, 0, stream>>>(a);
+    token_logprobs_bwd_kernel<T, kThreads><<<unsigned(a.rows) * unsigned(a.chunks), kThreads, 0, stream>>>(a);
     return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_backward(const BwdArgs& a, cudaStream_t stream) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a.logits), d = reinterpret_cast<uintptr_t>(a.dlogits);
+    const bool same_phase = ((x ^ d) & 15u) == 0 && ((a.row_stride - a.d_row_stride) * (long long)sizeof(T)) % 16 == 0;
+    if (a.V <= kWarpGradVocab || !same_phase) {
+        constexpr int rows = kWarpRowThreads / 32;
+        token_logprobs_bwd_warp_kernel<T><<<(a.rows + rows - 1) / rows, kWarpRowThreads, 0, stream>>>(a);
+        return cudaGetLastError();
+    }
+    return a.V <= kSmallRowVecs * Elem<T>::kPerVec ? launch_gradient<T, 64>(a, stream) : launch_gradient<T, 256>(a, stream);
 }
 
 }  // namespace
