@@ -2,11 +2,13 @@
 and lib/libb200attn.a (the same objects, for static linking in place of the reference's
 src/kernels/attention.cu); beside them the drop-ins for the callers of the path: lib/libb200gemm.a
 (src/kernels/matmul.cu), lib/libb200loss.so / .a (src/kernels/loss.cu) and lib/libb200norm.a
-(src/kernels/layernorm.cu), lib/libb200ffn.a (src/kernels/ffn.cu). Rebuilds only when a source is newer than the library."""
+(src/kernels/layernorm.cu), lib/libb200ffn.a (src/kernels/ffn.cu); and lib/_b200calls.so, the Python entry of the calls
+made once per layer and token. Rebuilds only when a source is newer than the library."""
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -23,6 +25,7 @@ NORM_AR = os.path.join(LIBDIR, "libb200norm.a")
 FFN_AR = os.path.join(LIBDIR, "libb200ffn.a")
 LOSS_SO = os.path.join(LIBDIR, "libb200loss.so")
 LOSS_AR = os.path.join(LIBDIR, "libb200loss.a")
+CALLS_SO = os.path.join(LIBDIR, "_b200calls.so")
 
 
 def _nvcc():
@@ -103,6 +106,18 @@ def build(verbose=False, force=False, ptxas_info=False):
         if os.path.exists(LOSS_AR):
             os.remove(LOSS_AR)
         subprocess.check_call(["ar", "rcs", LOSS_AR] + loss_objs)
+    # the Python entry of the calls made once per layer and token, over both libraries (found beside it at run time)
+    calls_src = os.path.join(HERE, "binding", "calls.cpp")
+    if force or _stale(CALLS_SO, [calls_src, os.path.join(HERE, "..", "include", "b200attn.h"), os.path.join(HERE, "..", "include", "b200loss.h")]):
+        import torch
+        t = os.path.dirname(torch.__file__)
+        subprocess.check_call(["g++", "-O2", "-std=c++17", "-Wall", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                               "-I", os.path.join(HERE, "..", "include"), "-isystem", os.path.join(t, "include"),
+                               "-isystem", os.path.join(t, "include", "torch", "csrc", "api", "include"),
+                               "-isystem", os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(nvcc))), "include"),
+                               "-I", sysconfig.get_path("include"), calls_src, "-o", CALLS_SO, "-L", os.path.join(t, "lib"),
+                               "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-lc10", "-lc10_cuda",
+                               "-L", LIBDIR, "-lb200attn", "-lb200loss", "-Wl,-rpath,$ORIGIN"])
     # the LayerNorm drop-in (static library only: its interface is the C++ header of the reference)
     norm_src = os.path.join(HERE, "norm", "layernorm_dropin.cu")
     norm_obj = os.path.join(OBJDIR, "layernorm_dropin.o")

@@ -901,8 +901,11 @@ extern "C" int b200attn_fwd_bf16_ragged(const void* q, const void* k, const void
     a.BH = H, a.T = total, a.d = d, a.H = H;
     a.scale = scale;
     a.fault_word = st->fault_word;
-    a.ragged = RaggedWork{s.items, s.count, s.capacity, H / Hkv, Hkv, out_stride};
-    RETURN_IF_CUDA(launch_ragged_plan(offsets, n, total, s.items, s.count, s.capacity, nullptr, stream), "work list launch");
+    // A list of work items is a launch of its own; where all CTAs fit the card at once (two per SM) and there are few sequences, each
+    // CTA finds its item itself.
+    const bool find = n <= kRaggedFindMax && (long long)s.capacity * H <= 2 * 148;
+    a.ragged = RaggedWork{offsets, n, find ? nullptr : s.items, s.count, s.capacity, H / Hkv, Hkv, out_stride};
+    if (!find) RETURN_IF_CUDA(launch_ragged_plan(a.ragged, total, stream), "work list launch");
     ScopedKernelTimer timer(0, stream);
     RETURN_IF_CUDA(launch_attn_fwd_ragged(a, stream), "packed forward launch");
     return B200ATTN_OK;
@@ -950,7 +953,7 @@ extern "C" int b200attn_bwd_bf16_ragged(const void* q, const void* k, const void
     a.scale = scale;
     a.fault_word = st->fault_word;
     a.grad_lt = dkv_stride, a.grad_lh = d, a.grad_lb = 0;
-    a.ragged = RaggedWork{s.items, s.count, s.capacity, H / Hkv, Hkv, dkv_stride};
+    a.ragged = RaggedWork{offsets, n, s.items, s.count, s.capacity, H / Hkv, Hkv, dkv_stride};
     BwdStatRows ext{nullptr, nullptr, 0.f};
     if (d == 64) {
         ext = BwdStatRows{s.lse_ext, s.d_ext, 1.0f / scale};
@@ -958,9 +961,8 @@ extern "C" int b200attn_bwd_bf16_ragged(const void* q, const void* k, const void
         if ((rc = make_stat_map(&a.map_d_ext, s.d_ext, 1, H, total))) return rc;
         a.work_counter = reinterpret_cast<unsigned int*>(s.count + 1);
     }
-    RETURN_IF_CUDA(launch_ragged_plan(offsets, n, total, s.items, s.count, s.capacity, a.work_counter, stream), "work list launch");
     RETURN_IF_CUDA(launch_ragged_prepass(static_cast<const __nv_bfloat16*>(out), out_stride, static_cast<const __nv_bfloat16*>(dout),
-                                         dout_stride, lse, s.D, s.lse2, s.dq_acc, total, H, d, ext, stream), "pre-pass");
+                                         dout_stride, lse, s.D, s.lse2, s.dq_acc, total, H, d, ext, a.ragged, stream), "pre-pass");
     {
         ScopedKernelTimer timer(1, stream);
         RETURN_IF_CUDA(d == 64 ? launch_attn_bwd_ragged64(a, stream) : launch_attn_bwd_ragged128(a, stream), "packed backward launch");

@@ -2,12 +2,13 @@
 // pre-pass over O and dO, and the conversion of the dQ sums. (The attention itself: the RAGGED instances of
 // attn_tc_fwd_short.cu, attn_tc_bwd.cu and attn_tc_bwd64.cu.)
 #include "kernels.cuh"
+#include "ragged_items.cuh"
 #include "tc_common.cuh"
 
 namespace b200attn {
 namespace {
 
-constexpr int kTile = 128;
+constexpr int kTile = kRaggedTile;
 constexpr float kLog2e = 1.4426950408889634f;
 
 // ------------------------------------------------------------------ work items
@@ -17,25 +18,20 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kPlanThreads = 1024;
 constexpr int kLevels = 4096;
 
-__device__ __forceinline__ int2 sequence_rows(const int* offsets, int i, int T) {  // first row and length, within [0, T]
-    const int a = min(max(offsets[i], 0), T), b = min(max(offsets[i + 1], a), T);
-    return make_int2(a, b - a);
-}
+struct PlanShared {
+    int level[kLevels];
+    int warp_total[32];
+    int total;
+};
 
-__global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(const int* __restrict__ offsets, int n, int T, int4* __restrict__ items,
-                                                                   int* __restrict__ count, int capacity, unsigned int* counter, int shift) {
-    __shared__ int level[kLevels];
-    __shared__ int warp_total[32];
-    __shared__ int s_levels;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    pdl_launch_dependents();
-    pdl_wait();
-    // Calls visit(first row, length, tiles) for every item of the sequences i = tid, tid + 1024, ...: short sequences by the
+__device__ void make_plan(const RaggedWork& w, int T, int shift, PlanShared& sh) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, threads = blockDim.x;
+    // Calls visit(first row, length, tiles) for every item of the sequences i = tid, tid + threads, ...: short sequences by the
     // thread that holds them, long ones by its whole warp.
     auto for_items = [&](auto&& visit) {
-        for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
+        for (int i0 = 0; i0 < w.n; i0 += threads) {
             const int i = i0 + tid;
-            const int2 s = i < n ? sequence_rows(offsets, i, T) : make_int2(0, 0);
+            const int2 s = i < w.n ? ragged_rows(w.offsets, i, T) : make_int2(0, 0);
             const int tiles = (s.y + kTile - 1) / kTile;
             if (tiles <= 8)
                 for (int c = 1; c <= tiles; ++c) visit(s.x, s.y, c);
@@ -49,56 +45,62 @@ __global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(const int* __
         }
     };
     const int levels = min(kLevels, (((T + kTile - 1) / kTile - 1) >> shift) + 1);
-    for (int i = tid; i < levels; i += kPlanThreads) level[i] = 0;
+    for (int i = tid; i < levels; i += threads) sh.level[i] = 0;
     __syncthreads();
     // level l (descending): position 0 is the longest
-    for_items([&](int, int, int c) { atomicAdd(&level[levels - 1 - ((c - 1) >> shift)], 1); });
+    for_items([&](int, int, int c) { atomicAdd(&sh.level[levels - 1 - ((c - 1) >> shift)], 1); });
     __syncthreads();
-    // exclusive prefix sum over the levels, kLevels / 1024 neighbours per thread
-    constexpr int kPer = kLevels / kPlanThreads;
-    int v[kPer], sum = 0;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const int at = tid * kPer + i;
-        v[i] = at < levels ? level[at] : 0;
-        sum += v[i];
-    }
+    // exclusive prefix sum over the levels, neighbours to one thread
+    const int per = (levels + threads - 1) / threads;
+    int sum = 0;
+    for (int i = tid * per; i < min(levels, (tid + 1) * per); ++i) sum += sh.level[i];
     int incl = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += y;
     }
-    if (lane == 31) warp_total[warp] = incl;
+    if (lane == 31) sh.warp_total[warp] = incl;
     __syncthreads();
     if (warp == 0) {
-        int x = warp_total[lane];
+        int x = lane < threads / 32 ? sh.warp_total[lane] : 0;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int y = __shfl_up_sync(0xffffffffu, x, o);
             if (lane >= o) x += y;
         }
-        warp_total[lane] = x;
-        if (lane == 31) s_levels = x;
+        sh.warp_total[lane] = x;
+        if (lane == 31) sh.total = x;
     }
     __syncthreads();
-    int at_item = incl - sum + (warp ? warp_total[warp - 1] : 0);
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        const int at = tid * kPer + i;
-        if (at < levels) level[at] = at_item;
-        at_item += v[i];
+    int at_item = incl - sum + (warp ? sh.warp_total[warp - 1] : 0);
+    for (int i = tid * per; i < min(levels, (tid + 1) * per); ++i) {
+        const int count = sh.level[i];
+        sh.level[i] = at_item;
+        at_item += count;
     }
     __syncthreads();
     // offsets that are not in ascending order could make more items than fit: those behind the list are dropped
     for_items([&](int row, int len, int c) {
-        const int at = atomicAdd(&level[levels - 1 - ((c - 1) >> shift)], 1);
-        if (at < capacity) items[at] = make_int4(row, len, c, 0);
+        const int at = atomicAdd(&sh.level[levels - 1 - ((c - 1) >> shift)], 1);
+        if (at < w.capacity) w.items[at] = make_int4(row, len, c, 0);
     });
     if (tid == 0) {
-        *count = min(s_levels, capacity);
-        if (counter) *counter = 0u;
+        w.count[0] = min(sh.total, w.capacity);
+        w.count[1] = 0;
     }
+}
+int plan_shift(int T) {
+    int shift = 0;
+    while ((((T + kTile - 1) / kTile - 1) >> shift) >= kLevels) ++shift;
+    return shift;
+}
+
+__global__ void __launch_bounds__(kPlanThreads) ragged_plan_kernel(const RaggedWork w, int T, int shift) {
+    __shared__ PlanShared sh;
+    pdl_launch_dependents();
+    pdl_wait();
+    make_plan(w, T, shift, sh);
 }
 
 // ------------------------------------------------------------------ pre-pass
@@ -108,11 +110,16 @@ __global__ void __launch_bounds__(256) ragged_prepass_kernel(const __nv_bfloat16
                                                              const __nv_bfloat16* __restrict__ dO, long long do_stride,
                                                              const float* __restrict__ lse, float* __restrict__ Dout,
                                                              float* __restrict__ lse2, float* __restrict__ dq_acc, int T, int H, int d,
-                                                             BwdStatRows ext) {
+                                                             BwdStatRows ext, const RaggedWork w, int shift) {
+    __shared__ PlanShared sh;
     pdl_launch_dependents();
     pdl_wait();
+    if (blockIdx.x == 0) {  // first, so that it does not end last
+        make_plan(w, T, shift, sh);
+        return;
+    }
     const int tpr = d / 8;
-    const long long gid = blockIdx.x * 256ll + threadIdx.x;
+    const long long gid = (blockIdx.x - 1) * 256ll + threadIdx.x;
     const long long row = gid / tpr;  // t * H + h
     const int e = int(gid % tpr) * 8;
     const bool live = row < (long long)T * H;
@@ -165,20 +172,17 @@ __global__ void __launch_bounds__(256) ragged_dq_convert_kernel(const float* __r
 
 }  // namespace
 
-cudaError_t launch_ragged_plan(const int* offsets, int n, int T, int4* items, int* count, int capacity, unsigned int* counter,
-                               cudaStream_t stream) {
-    int shift = 0;
-    while ((((T + kTile - 1) / kTile - 1) >> shift) >= kLevels) ++shift;
-    return launch_pdl(ragged_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, offsets, n, T, items, count, capacity, counter, shift);
+cudaError_t launch_ragged_plan(const RaggedWork& w, int T, cudaStream_t stream) {
+    return launch_pdl(ragged_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, w, T, plan_shift(T));
 }
 
 cudaError_t launch_ragged_prepass(const __nv_bfloat16* o, long long o_stride, const __nv_bfloat16* dO, long long do_stride,
                                   const float* lse, float* D, float* lse2, float* dq_acc, int T, int H, int d, BwdStatRows ext,
-                                  cudaStream_t stream) {
-    const long long blocks = ((long long)T * H * (d / 8) + 255) / 256;
+                                  const RaggedWork& w, cudaStream_t stream) {
+    const long long blocks = ((long long)T * H * (d / 8) + 255) / 256 + 1;
     if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
     return launch_pdl(ragged_prepass_kernel, dim3((unsigned int)blocks), dim3(256), 0, stream, o, o_stride, dO, do_stride, lse, D, lse2,
-                      dq_acc, T, H, d, ext);
+                      dq_acc, T, H, d, ext, w, plan_shift(T));
 }
 
 cudaError_t launch_ragged_dq_convert(const float* dq_acc, __nv_bfloat16* dq, long long dq_stride, const int* offsets, int n, int T,

@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc_kernel(const __grid_c
     pdl_wait();
     if constexpr (RAGGED) {
         const int item = int(blockIdx.x / unsigned(a.ragged.kv_heads));
-        if (item >= *a.ragged.count) {
+        if (item >= a.ragged.count[0]) {  // the host knows an upper bound only
             __syncthreads();
             if (warp == kProducerWarp) tmem_dealloc(tmem, Cfg::kTmemCols);
             return;

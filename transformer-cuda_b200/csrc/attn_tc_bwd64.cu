@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc64_kernel(const __grid
             tma_prefetch_desc(&a.map_lse_ext);
             tma_prefetch_desc(&a.map_d_ext);
             int published = 0;
-            const int n_items = RAGGED ? *a.ragged.count * a.ragged.kv_heads : total_items;
+            const int n_items = RAGGED ? a.ragged.count[0] * a.ragged.kv_heads : total_items;
             auto publish_next = [&]() {
                 int w = int(atomicAdd(a.work_counter, 1u));
                 if (w >= n_items) w = -1;

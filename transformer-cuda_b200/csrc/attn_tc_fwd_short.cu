@@ -35,6 +35,7 @@
 // Every mbarrier wait has an iteration limit (tc_common.cuh); a wait that gives up sets the fault
 // word and the kernel still runs to its end and frees its TMEM.
 #include "kernels.cuh"
+#include "ragged_items.cuh"
 #include "tc_common.cuh"
 
 
@@ -126,12 +127,14 @@ __global__ void __launch_bounds__(kThreads, 2) attn_fwd_tc_short_kernel(const __
     pdl_wait();
     if constexpr (RAGGED) {  // the heads of one tile are neighbours: those of a group read the same key tiles
         const int item = int(blockIdx.x / unsigned(a.H));
-        if (item >= *a.ragged.count) {
+        int4 w = make_int4(0, 0, 0, 0);
+        if (a.ragged.items == nullptr) w = ragged_find(a.ragged.offsets, a.ragged.n, a.T, item, lane);
+        else if (item < a.ragged.count[0]) w = a.ragged.items[item];
+        if (w.z == 0) {  // the host knows an upper bound only
             __syncthreads();
             if (warp == 4) tmem_dealloc(tmem, Cfg::kTmemCols);
             return;
         }
-        const int4 w = a.ragged.items[item];
         bh = hh = int(blockIdx.x % unsigned(a.H)), hk = hh / a.ragged.group;
         row0 = w.x, qt = w.z - 1, valid = min(kBM, w.y - qt * kBM);
     }

@@ -89,16 +89,18 @@ cudaError_t launch_attn_bwd_f32_tiled(const float* q, const float* k, const floa
 // tiles the item walks per head. The forward's item is query tile `tiles - 1` (key tiles 0 .. tiles - 1), the backward's key
 // tile n - tiles of the sequence's n (query tiles from there to the last). Items are in descending order of `tiles`.
 struct RaggedWork {
-    const int4* items;
-    const int* count;     // number of items (device)
-    int capacity;         // upper bound of it known to the host
+    const int* offsets;   // n + 1 of them (device); clipped to [0, T]
+    int n;
+    int4* items;          // NULL: every CTA finds its item in the offsets itself (forward, n <= kRaggedFindMax)
+    int* count;           // [0] number of items, [1] work counter of the persistent backward (device)
+    int capacity;         // upper bound of the number of items, known to the host
     int group;            // query heads per key head
     int kv_heads;
     long long out_stride; // element stride between rows of `out` (forward) or of dk and dv (backward)
 };
-// Writes items and count from the n + 1 offsets (device), clipped to [0, T], and clears *counter.
-cudaError_t launch_ragged_plan(const int* offsets, int n, int T, int4* items, int* count, int capacity, unsigned int* counter,
-                               cudaStream_t stream);
+constexpr int kRaggedFindMax = 128;
+// Writes items and count and clears the work counter.
+cudaError_t launch_ragged_plan(const RaggedWork& w, int T, cudaStream_t stream);
 
 struct TcFwdArgs {
     CUtensorMap map_q, map_k, map_v, map_o;  // BF16
@@ -176,10 +178,11 @@ cudaError_t launch_dq_convert_strided(const float* dq_acc, __nv_bfloat16* dq, lo
 cudaError_t launch_dq_convert(const float* dq_acc, __nv_bfloat16* dq, long long n, cudaStream_t stream, float scale = 1.0f);
 
 // ------------------------------------------------------------------ attn_ragged.cu (passes around the kernels for packed sequences)
-// D, lse2 (and, with ext, the statistics rows) of all T x H rows, (H, T); clears the (T, H, d) FP32 accumulator dq_acc.
+// D, lse2 (and, with ext, the statistics rows) of all T x H rows, (H, T); clears the (T, H, d) FP32 accumulator dq_acc; and,
+// in one CTA beside that, what launch_ragged_plan does.
 cudaError_t launch_ragged_prepass(const __nv_bfloat16* o, long long o_stride, const __nv_bfloat16* dO, long long do_stride,
                                   const float* lse, float* D, float* lse2, float* dq_acc, int T, int H, int d, BwdStatRows ext,
-                                  cudaStream_t stream);
+                                  const RaggedWork& w, cudaStream_t stream);
 // dq (BF16 rows at dq_stride) = dq_acc * scale for the rows offsets[0] .. offsets[n] (clipped to [0, T]); others keep their values.
 cudaError_t launch_ragged_dq_convert(const float* dq_acc, __nv_bfloat16* dq, long long dq_stride, const int* offsets, int n, int T,
                                      int H, int d, float scale, cudaStream_t stream);

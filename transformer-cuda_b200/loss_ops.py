@@ -6,11 +6,10 @@ sarimahsan/transformer-cuda with torch CUDA tensors in place of raw pointers. `t
 missing library raises."""
 import collections
 import ctypes
-import math
 import os
 import re
 
-import torch
+from . import calls as _calls
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 SO_PATH = os.path.join(HERE, "lib", "libb200loss.so")
@@ -63,6 +62,7 @@ def _check(code):
 def cross_entropy_forward_backward(logits, targets, dlogits=None, want_loss=True):
     """logits (B, T, V) float32, targets (B, T) int32 -> (dlogits, loss): dlogits = (softmax - onehot) / (B*T) and
     loss a 0-d CUDA tensor holding the mean (None when `want_loss` is false). Asynchronous on the current stream."""
+    import torch
     if logits.dtype != torch.float32 or not logits.is_cuda or not logits.is_contiguous() or logits.dim() != 3:
         raise ValueError("logits must be a contiguous CUDA float32 tensor of shape (B, T, V)")
     B, T, V = logits.shape
@@ -81,43 +81,6 @@ def cross_entropy_forward_backward(logits, targets, dlogits=None, want_loss=True
 
 
 TokenLogprobs = collections.namedtuple("TokenLogprobs", "logprobs entropy stats top_logprobs top_tokens temperature")
-MAX_TOP = 32
-
-
-_DTYPES = {torch.float32: 0, torch.bfloat16: 1}  # B200LOSS_F32, B200LOSS_BF16
-
-
-def _rows(t, name):
-    """(rows, V, row stride) of FP32 or BF16 rows (..., V): contiguous elements, one stride from row to row."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in _DTYPES or t.dim() < 1 or t.shape[-1] < 1:
-        raise ValueError(f"{name} must be a CUDA float32 or bfloat16 tensor of shape (..., V)")
-    shape, strides = t.shape, t.stride()
-    V = shape[-1]
-    if len(shape) == 2:
-        rows, stride, regular = shape[0], strides[0] if shape[0] > 1 else V, True
-    else:
-        lead = [(n, st) for n, st in zip(shape[:-1], strides[:-1]) if n != 1]
-        rows, stride = math.prod(shape[:-1]), lead[-1][1] if lead else V
-        regular = all(a[1] == b[0] * b[1] for a, b in zip(lead, lead[1:]))
-    if rows and ((strides[-1] != 1 and V > 1) or not regular or stride < V):
-        raise ValueError(f"{name} must consist of contiguous rows at one row stride (strides {strides})")
-    return rows, V, stride
-
-
-def _per_row(t, name, dtype, device, rows):
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.get_device() != device or t.numel() != rows or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor on the logits' device with one element per row ({rows})")
-    return t.data_ptr()
-
-
-def _call(name, device, *args):
-    """The C call on the current stream of `device`; the device is only switched where it is not the current one."""
-    fn = getattr(load(), name)
-    if device == torch.cuda.current_device():
-        _check(fn(*args, torch._C._cuda_getCurrentRawStream(device)))
-    else:
-        with torch.cuda.device(device):
-            _check(fn(*args, torch._C._cuda_getCurrentRawStream(device)))
 
 
 def token_logprobs_forward(logits, targets, temperature=1.0, top=0):
@@ -129,46 +92,15 @@ def token_logprobs_forward(logits, targets, temperature=1.0, top=0):
     Returns TokenLogprobs: logprobs, entropy (...) and stats (..., 2) float32, top_logprobs (..., top) float32 and top_tokens
     (..., top) int32 (None when top = 0; larger logits first, equal ones by the lower index; top <= min(32, V)), and the
     temperature. -inf logits are tokens that are not allowed; see include/b200loss.h for rows without any and for NaN."""
-    rows, V, stride = _rows(logits, "logits")
-    dev, index = logits.device, logits.get_device()
-    t_ptr = _per_row(targets, "targets", torch.int32, index, rows)
-    if not 0 <= top <= min(MAX_TOP, V):
-        raise ValueError(f"top must be between 0 and min({MAX_TOP}, V), got {top}")
-    lead, f32 = logits.shape[:-1], torch.float32
-    logprobs, entropy = torch.empty(lead, dtype=f32, device=dev), torch.empty(lead, dtype=f32, device=dev)
-    stats = torch.empty((*lead, 2), dtype=f32, device=dev)
-    top_logprobs = top_tokens = p_ptr = k_ptr = None
-    if top:
-        top_logprobs = torch.empty((*lead, top), dtype=f32, device=dev)
-        top_tokens = torch.empty((*lead, top), dtype=torch.int32, device=dev)
-        p_ptr, k_ptr = top_logprobs.data_ptr(), top_tokens.data_ptr()
-    _call("b200loss_token_logprobs", index, logits.data_ptr(), _DTYPES[logits.dtype], stride, t_ptr, rows, V, temperature,
-          logprobs.data_ptr(), entropy.data_ptr(), stats.data_ptr(), top, p_ptr, k_ptr)
-    return TokenLogprobs(logprobs, entropy, stats, top_logprobs, top_tokens, temperature)
+    return TokenLogprobs(*_calls.load().token_logprobs(logits, targets, temperature, top), temperature)
 
 
 def token_logprobs_backward(logits, targets, result, grad_logprobs, grad_entropy=None, dlogits=None):
     """Gradient of sum(grad_logprobs * logprobs + grad_entropy * entropy) with regard to the logits that
     `token_logprobs_forward(logits, targets, ...)` returned `result` for. grad_* (...) float32; dlogits: the logits' shape and
     type, allocated when not given, may be `logits` itself. Rows that no gradient reaches are zeros."""
-    rows, V, stride = _rows(logits, "logits")
-    index, f32 = logits.get_device(), torch.float32
-    t_ptr = _per_row(targets, "targets", torch.int32, index, rows)
-    e_ptr = _per_row(result.entropy, "result.entropy", f32, index, rows)
-    s_ptr = _per_row(result.stats, "result.stats", f32, index, 2 * rows)
-    g_ptr = _per_row(grad_logprobs, "grad_logprobs", f32, index, rows)
-    ge_ptr = None if grad_entropy is None else _per_row(grad_entropy, "grad_entropy", f32, index, rows)
-    if dlogits is None:
-        dlogits, d_stride = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device), V
-    else:
-        _, _, d_stride = _rows(dlogits, "dlogits")
-        if dlogits.dtype != logits.dtype or dlogits.get_device() != index or dlogits.shape != logits.shape:
-            raise ValueError("dlogits must have the logits' shape, type and device")
-        if dlogits.data_ptr() == logits.data_ptr() and d_stride != stride:
-            raise ValueError("dlogits in the logits' place must have the logits' row stride")
-    _call("b200loss_token_logprobs_backward", index, logits.data_ptr(), _DTYPES[logits.dtype], stride, t_ptr, e_ptr, s_ptr, g_ptr,
-          ge_ptr, rows, V, result.temperature, dlogits.data_ptr(), d_stride)
-    return dlogits
+    return _calls.load().token_logprobs_backward(logits, targets, result.entropy, result.stats, grad_logprobs, grad_entropy,
+                                                 result.temperature, dlogits)
 
 
 def kernel_path(logits, dlogits):

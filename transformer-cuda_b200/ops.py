@@ -11,6 +11,7 @@ import ctypes
 
 import torch
 
+from . import calls as _calls
 from . import lib as _lib
 
 
@@ -200,101 +201,19 @@ def attention_backward_bf16_packed(qkv, out, dout, lse, H, scale, dqkv=None):
     return dqkv
 
 
-def _fail(text):
-    raise _lib.B200AttnError(_lib.ERR_INVALID_ARGUMENT, text)
-
-
-def _head_rows(t, name, device, shape=None):
-    """Row stride of a BF16 tensor (rows, heads, d) on CUDA device `device` whose heads are contiguous; rows may be any distance
-    apart. `shape`: what it has to be."""
-    if not isinstance(t, torch.Tensor) or t.dtype != BF16 or t.dim() != 3 or t.get_device() != device:
-        _fail(f"{name}: expected a BF16 tensor (rows, heads, d) on CUDA device {device}")
-    s = t.shape
-    if shape is not None and s != shape:
-        _fail(f"{name}: has shape {tuple(s)}, expected {tuple(shape)}")
-    rows, heads, d = s
-    st = t.stride()
-    if (st[2] != 1 and d > 1 or st[1] != d and heads > 1) and rows and heads:
-        _fail(f"{name}: heads must be contiguous (strides {st})")
-    return st[0] if rows > 1 else heads * d
-
-
-def _vector(t, name, dtype, numel, device):
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.get_device() != device or t.numel() != numel or not t.is_contiguous():
-        _fail(f"{name}: expected a contiguous {dtype} tensor of {numel} elements on CUDA device {device}")
-    return t.data_ptr()
-
-
-def _device_of(t, name):
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        _fail(f"{name}: expected a CUDA tensor")
-    return t.get_device()
-
-
-def _call_on(device, name, *args):
-    """The C call on the current stream of `device`; the device is only switched where it is not the current one."""
-    fn = getattr(_lib.load(), name)
-    if device == torch.cuda.current_device():
-        _lib.check(fn(*args, torch._C._cuda_getCurrentRawStream(device)))
-    else:
-        with torch.cuda.device(device):
-            _lib.check(fn(*args, torch._C._cuda_getCurrentRawStream(device)))
-
-
-def _workspace(nbytes, like):
-    """Scratch of one call from torch's allocator: ordered with the stream, its own in every captured graph."""
-    return torch.empty(nbytes if nbytes > 16 else 16, dtype=torch.uint8, device=like.device)
-
-
-def _ragged_shapes(q, k, v, offsets):
-    device = _device_of(q, "q")
-    sq = _head_rows(q, "q", device)
-    total, H, d = q.shape
-    skv = _head_rows(k, "k", device)
-    rows_k, Hkv, d_k = k.shape
-    if rows_k != total or d_k != d or Hkv == 0 or H % Hkv != 0:
-        _fail(f"k: expected ({total}, a divisor of {H}, {d}), got {tuple(k.shape)}")
-    if _head_rows(v, "v", device, k.shape) != skv:
-        _fail("k and v must have the same row stride")
-    if not isinstance(offsets, torch.Tensor) or offsets.dim() != 1 or offsets.numel() < 1:
-        _fail("offsets: expected a tensor of n + 1 row numbers")
-    n = offsets.numel() - 1
-    return device, total, n, H, Hkv, d, sq, skv, _vector(offsets, "offsets", torch.int32, n + 1, device)
-
-
 def attention_forward_bf16_ragged(q, k, v, offsets, scale, out=None, lse=None):
     """Causal attention over packed sequences of different lengths with grouped heads. q (total, H, d), k and v
     (total, Hkv, d) BF16 with H a multiple of Hkv, contiguous heads and any row stride that is a multiple of 8 (the parts of
     a fused projection output will do); offsets int32 (n + 1) on the same device: sequence i is rows offsets[i] ..
     offsets[i + 1] - 1. Returns (out (total, H, d) BF16, lse (H, total) FP32). Rows that belong to no sequence are left as
     they are in `out` and `lse` when these are given, and are zero when they are allocated here."""
-    device, total, n, H, Hkv, d, sq, skv, o_ptr = _ragged_shapes(q, k, v, offsets)
-    out = torch.zeros(total, H, d, dtype=BF16, device=q.device) if out is None else out
-    lse = torch.zeros(H, total, dtype=F32, device=q.device) if lse is None else lse
-    so = _head_rows(out, "out", device, q.shape)
-    lse_ptr = _vector(lse, "lse", F32, H * total, device)
-    nbytes = _lib.load().b200attn_ragged_workspace_bytes(total, n, H, d, 0)
-    ws = _workspace(nbytes, q)
-    _call_on(device, "b200attn_fwd_bf16_ragged", q.data_ptr(), k.data_ptr(), v.data_ptr(), o_ptr, out.data_ptr(), lse_ptr, ws.data_ptr(),
-             nbytes, total, n, H, Hkv, d, sq, skv, so, scale)
-    return out, lse
+    return _calls.load().ragged_forward(q, k, v, offsets, scale, out, lse)
 
 
 def attention_backward_bf16_ragged(q, k, v, out, dout, lse, offsets, scale, dq=None, dk=None, dv=None):
     """Backward of attention_forward_bf16_ragged: dout (total, H, d) BF16 -> (dq, dk, dv), overwritten for the rows of the
     sequences (dk and dv summed over the heads of a group); other rows as in the forward. dk and dv share a row stride."""
-    device, total, n, H, Hkv, d, sq, skv, o_ptr = _ragged_shapes(q, k, v, offsets)
-    so, sdo = _head_rows(out, "out", device, q.shape), _head_rows(dout, "dout", device, q.shape)
-    lse_ptr = _vector(lse, "lse", F32, H * total, device)
-    dq, dk, dv = (torch.zeros(x.shape, dtype=BF16, device=q.device) if t is None else t for t, x in ((dq, q), (dk, k), (dv, v)))
-    sdq, sdk = _head_rows(dq, "dq", device, q.shape), _head_rows(dk, "dk", device, k.shape)
-    if _head_rows(dv, "dv", device, k.shape) != sdk:
-        _fail("dk and dv must have the same row stride")
-    nbytes = _lib.load().b200attn_ragged_workspace_bytes(total, n, H, d, 1)
-    ws = _workspace(nbytes, q)
-    _call_on(device, "b200attn_bwd_bf16_ragged", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dout.data_ptr(), lse_ptr, o_ptr,
-             dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), nbytes, total, n, H, Hkv, d, sq, skv, so, sdo, sdq, sdk, scale)
-    return dq, dk, dv
+    return _calls.load().ragged_backward(q, k, v, out, dout, lse, offsets, scale, dq, dk, dv)
 
 
 def attention_decode_bf16(q, k_cache, v_cache, lengths, scale, out=None, lse=None):
@@ -302,32 +221,7 @@ def attention_decode_bf16(q, k_cache, v_cache, lengths, scale, out=None, lse=Non
     (B, T, Hkv, d) BF16 with contiguous d and any other strides that are multiples of 8 (a (B, Hkv, T, d) cache goes in
     transposed); lengths int32 (B): keys that the token of sequence b sees, its own included. Returns (out (B, H, d) BF16,
     lse (B, H) FP32); a sequence of length 0 gets zeros and -inf. Rows behind a length are never read."""
-    device = _device_of(q, "q")
-    sq = _head_rows(q, "q", device)
-    B, H, d = q.shape
-    for t, nm in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        if not isinstance(t, torch.Tensor) or t.dtype != BF16 or t.dim() != 4 or t.get_device() != device:
-            _fail(f"{nm}: expected a BF16 tensor (B, T, Hkv, d) on CUDA device {device}")
-    shape = k_cache.shape
-    T, Hkv = shape[1], shape[2]
-    if shape[0] != B or shape[3] != d or Hkv == 0 or H % Hkv != 0 or v_cache.shape != shape:
-        _fail(f"k_cache, v_cache: expected ({B}, T, a divisor of {H}, {d}), got {tuple(shape)} and {tuple(v_cache.shape)}")
-    strides = []
-    for t in (k_cache, v_cache):
-        b, r, h, e = t.stride()
-        if e != 1 and T:
-            _fail("k_cache, v_cache: the last dimension must be contiguous")
-        # a dimension of one element has no stride to keep
-        strides += (b if B > 1 else 0, r if T > 1 else 0, h if Hkv > 1 else 0)
-    n_ptr = _vector(lengths, "lengths", torch.int32, B, device)
-    out = torch.empty(B, H, d, dtype=BF16, device=q.device) if out is None else out
-    lse = torch.empty(B, H, dtype=F32, device=q.device) if lse is None else lse
-    o_ptr, lse_ptr = _vector(out, "out", BF16, B * H * d, device), _vector(lse, "lse", F32, B * H, device)
-    nbytes = _lib.load().b200attn_decode_workspace_bytes(B, T, H, Hkv, d)
-    ws = _workspace(nbytes, q)
-    _call_on(device, "b200attn_decode_bf16", q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), n_ptr, o_ptr, lse_ptr, ws.data_ptr(), nbytes,
-             B, T, H, Hkv, d, sq, *strides, scale)
-    return out, lse
+    return _calls.load().decode(q, k_cache, v_cache, lengths, scale, out, lse)
 
 
 def qkv_split_transpose_forward_bf16(qkv, q, k, v, B, T, H, d_head):
