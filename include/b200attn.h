@@ -182,16 +182,16 @@ int b200attn_bwd_bf16_noalloc(const void* q, const void* k, const void* v, const
  * of its own sequence up to itself. out (total, H, d) BF16, lse (H, total) FP32. Heads are contiguous (stride d), rows are
  * *_stride elements apart (a multiple of 8), so q, k and v may be parts of one projection output. Rows that belong to no sequence
  * are not read into any result and keep their values in out and lse. d in {64, 128}, scale > 0; 16-byte aligned tensors.
- * `workspace` (caller-owned, b200attn_ragged_workspace_bytes(total, n, H, d, 0) bytes, 16-byte aligned) is written by the
+ * `workspace` (caller-owned, b200attn_ragged_workspace_bytes(total, n, H, Hkv, d, 0) bytes, 16-byte aligned) is written by the
  * call; calls that may run at the same time need workspaces of their own. No counterpart in the reference. */
-long long b200attn_ragged_workspace_bytes(int total, int n, int H, int d, int backward);
+long long b200attn_ragged_workspace_bytes(int total, int n, int H, int Hkv, int d, int backward);
 int b200attn_fwd_bf16_ragged(const void* q, const void* k, const void* v, const int* offsets, void* out, float* lse,
                              void* workspace, long long workspace_bytes, int total, int n, int H, int Hkv, int d,
                              long long q_stride, long long kv_stride, long long out_stride, float scale,
                              b200attn_stream_t stream);
 /* Its backward: dq (total, H, d), dk and dv (total, Hkv, d) BF16 of the rows that belong to a sequence, overwritten (dk and
  * dv summed over the query heads of a group), from the forward's out and lse and from dout (total, H, d). Workspace:
- * b200attn_ragged_workspace_bytes(total, n, H, d, 1) bytes. dQ is summed in FP32 in an order that is not fixed, like that of
+ * b200attn_ragged_workspace_bytes(total, n, H, Hkv, d, 1) bytes. dQ is summed in FP32 in an order that is not fixed, like that of
  * b200attn_bwd_bf16. */
 int b200attn_bwd_bf16_ragged(const void* q, const void* k, const void* v, const void* out, const void* dout, const float* lse,
                              const int* offsets, void* dq, void* dk, void* dv, void* workspace, long long workspace_bytes,

@@ -38,7 +38,7 @@ LENGTHS = [[1], [5], [128], [129], [1, 1, 1], [0, 5, 0, 130, 0], [127, 128, 129]
 
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("lengths", LENGTHS, ids=lambda x: "-".join(map(str, x)))
-@pytest.mark.parametrize("H,Hkv", [(1, 1), (4, 2), (6, 1)])
+@pytest.mark.parametrize("H,Hkv", [(1, 1), (4, 2), (6, 1), (21, 3)])
 def test_forward_and_backward(pkg, lengths, H, Hkv, d):
     q, k, v, dout, offsets = make(lengths, H, Hkv, d, seed=len(lengths) * 7 + H)
     scale = 1.0 / math.sqrt(d)

@@ -176,7 +176,7 @@ PyObject* ragged_forward(PyObject*, PyObject* const* p, Py_ssize_t np) {
             void* out_ptr;
             const int64_t so = head_rows_like(out, "out", *a.q, &out_ptr);
             float* lse_ptr = static_cast<float*>(vector(lse, Kind::kAttn, "lse", at::kFloat, (int64_t)a.H * a.total, device));
-            const long long bytes = b200attn_ragged_workspace_bytes(a.total, a.n, a.H, a.d, 0);
+            const long long bytes = b200attn_ragged_workspace_bytes(a.total, a.n, a.H, a.Hkv, a.d, 0);
             const at::Tensor ws = scratch(bytes, device);
             check_attn(b200attn_fwd_bf16_ragged(a.q->data_ptr(), a.k->data_ptr(), a.v->data_ptr(), static_cast<int*>(a.offsets), out_ptr, lse_ptr,
                                                 ws.data_ptr(), bytes, a.total, a.n, a.H, a.Hkv, a.d, a.sq, a.skv, so, scale,
@@ -207,7 +207,7 @@ PyObject* ragged_backward(PyObject*, PyObject* const* p, Py_ssize_t np) {
         try {
             const int64_t sdq = head_rows_like(dq, "dq", *a.q, &dq_ptr), sdk = head_rows_like(dk, "dk", *a.k, &dk_ptr);
             if (head_rows_like(dv, "dv", *a.k, &dv_ptr) != sdk) refuse(Kind::kAttn, "dk and dv must have the same row stride");
-            const long long bytes = b200attn_ragged_workspace_bytes(a.total, a.n, a.H, a.d, 1);
+            const long long bytes = b200attn_ragged_workspace_bytes(a.total, a.n, a.H, a.Hkv, a.d, 1);
             const at::Tensor ws = scratch(bytes, device);
             check_attn(b200attn_bwd_bf16_ragged(a.q->data_ptr(), a.k->data_ptr(), a.v->data_ptr(), out_ptr, dout_ptr, lse_ptr,
                                                 static_cast<int*>(a.offsets), dq_ptr, dk_ptr, dv_ptr, ws.data_ptr(), bytes, a.total, a.n, a.H,

@@ -823,11 +823,12 @@ struct RaggedSpace {
     int capacity;  // work items at most
     int4* items;
     int* count;              // [0] number of items, [1] work counter of the persistent backward
-    float *dq_acc, *D, *lse2;
+    float *dq_acc, *D, *lse2, *part_dk, *part_dv;
     __nv_bfloat16 *lse_ext, *d_ext;
+    int parts, part_heads;   // the heads of a group in the backward (RaggedWork)
     size_t bytes;
 };
-RaggedSpace ragged_space(void* base, int total, int n, int H, int d, bool backward) {
+RaggedSpace ragged_space(void* base, int total, int n, int H, int Hkv, int d, bool backward) {
     RaggedSpace s{};
     const long long tiles = (long long)total / 128 + n;  // every sequence adds at most one tile that is not full
     s.capacity = int(tiles < total ? tiles : total);
@@ -842,6 +843,16 @@ RaggedSpace ragged_space(void* base, int total, int n, int H, int d, bool backwa
         if (d == 64) {
             s.lse_ext = bump.take<__nv_bfloat16>(rows * 16);
             s.d_ext = bump.take<__nv_bfloat16>(rows * 16);
+        }
+        // Where the key tiles of the key heads do not fill the card twice over, the heads of a group are shared out.
+        const int group = H / Hkv;
+        const long long items = (long long)s.capacity * Hkv;
+        const long long want = items > 0 ? (2 * 148 + items - 1) / items : 1;
+        s.part_heads = want >= group ? 1 : int((group + want - 1) / want);
+        s.parts = (group + s.part_heads - 1) / s.part_heads;
+        if (s.parts > 1) {
+            s.part_dk = bump.take<float>(size_t(s.parts) * total * Hkv * d);
+            s.part_dv = bump.take<float>(size_t(s.parts) * total * Hkv * d);
         }
     }
     s.bytes = size_t(bump.p - static_cast<uint8_t*>(base));
@@ -863,9 +874,9 @@ Layout ragged_layout(long long stride, int d) { return Layout{stride, d, stride}
 
 }  // namespace
 
-extern "C" long long b200attn_ragged_workspace_bytes(int total, int n, int H, int d, int backward) {
-    if (total < 0 || n < 0 || H <= 0 || d <= 0) return 0;
-    return (long long)ragged_space(nullptr, total, n, H, d, backward != 0).bytes;
+extern "C" long long b200attn_ragged_workspace_bytes(int total, int n, int H, int Hkv, int d, int backward) {
+    if (total < 0 || n < 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || d <= 0) return 0;
+    return (long long)ragged_space(nullptr, total, n, H, Hkv, d, backward != 0).bytes;
 }
 
 extern "C" int b200attn_fwd_bf16_ragged(const void* q, const void* k, const void* v, const int* offsets, void* out, float* lse,
@@ -883,7 +894,7 @@ extern "C" int b200attn_fwd_bf16_ragged(const void* q, const void* k, const void
         return fail(B200ATTN_ERR_INVALID_ARGUMENT, "%s: tensors and workspace must be 16-byte aligned", fn);
     if (!row_stride_ok(q_stride, (long long)H * d) || !row_stride_ok(kv_stride, (long long)Hkv * d) || !row_stride_ok(out_stride, (long long)H * d))
         return fail(B200ATTN_ERR_INVALID_ARGUMENT, "%s: a row stride is smaller than its heads, not a multiple of 8 elements or too large", fn);
-    const RaggedSpace s = ragged_space(workspace, total, n, H, d, false);
+    const RaggedSpace s = ragged_space(workspace, total, n, H, Hkv, d, false);
     if (workspace_bytes < (long long)s.bytes)
         return fail(B200ATTN_ERR_SCRATCH, "%s: workspace of %lld bytes, needs %zu (b200attn_ragged_workspace_bytes)", fn, workspace_bytes, s.bytes);
     if ((long long)s.capacity * H > 0x7fffffffLL) return fail(B200ATTN_ERR_UNSUPPORTED, "%s: too many tiles", fn);
@@ -904,7 +915,7 @@ extern "C" int b200attn_fwd_bf16_ragged(const void* q, const void* k, const void
     // A list of work items is a launch of its own; where all CTAs fit the card at once (two per SM) and there are few sequences, each
     // CTA finds its item itself.
     const bool find = n <= kRaggedFindMax && (long long)s.capacity * H <= 2 * 148;
-    a.ragged = RaggedWork{offsets, n, find ? nullptr : s.items, s.count, s.capacity, H / Hkv, Hkv, out_stride};
+    a.ragged = RaggedWork{offsets, n, find ? nullptr : s.items, s.count, s.capacity, H / Hkv, Hkv, 1, H / Hkv, nullptr, nullptr, out_stride};
     if (!find) RETURN_IF_CUDA(launch_ragged_plan(a.ragged, total, stream), "work list launch");
     ScopedKernelTimer timer(0, stream);
     RETURN_IF_CUDA(launch_attn_fwd_ragged(a, stream), "packed forward launch");
@@ -930,10 +941,10 @@ extern "C" int b200attn_bwd_bf16_ragged(const void* q, const void* k, const void
     if (!row_stride_ok(q_stride, wq) || !row_stride_ok(kv_stride, wk) || !row_stride_ok(out_stride, wq) || !row_stride_ok(dout_stride, wq) ||
         !row_stride_ok(dq_stride, wq) || !row_stride_ok(dkv_stride, wk))
         return fail(B200ATTN_ERR_INVALID_ARGUMENT, "%s: a row stride is smaller than its heads, not a multiple of 8 elements or too large", fn);
-    const RaggedSpace s = ragged_space(workspace, total, n, H, d, true);
+    const RaggedSpace s = ragged_space(workspace, total, n, H, Hkv, d, true);
     if (workspace_bytes < (long long)s.bytes)
         return fail(B200ATTN_ERR_SCRATCH, "%s: workspace of %lld bytes, needs %zu (b200attn_ragged_workspace_bytes)", fn, workspace_bytes, s.bytes);
-    if ((long long)s.capacity * Hkv > 0x7fffffffLL || (long long)total * H * (d / 8) / 256 > 0x7ffffff0LL)
+    if ((long long)s.capacity * Hkv * s.parts > 0x7fffffffLL || (long long)total * H * (d / 8) / 256 > 0x7ffffff0LL)
         return fail(B200ATTN_ERR_UNSUPPORTED, "%s: too many tiles", fn);
     DeviceState* st = nullptr;
     if ((rc = device_state(stream, &st))) return rc;
@@ -953,7 +964,7 @@ extern "C" int b200attn_bwd_bf16_ragged(const void* q, const void* k, const void
     a.scale = scale;
     a.fault_word = st->fault_word;
     a.grad_lt = dkv_stride, a.grad_lh = d, a.grad_lb = 0;
-    a.ragged = RaggedWork{offsets, n, s.items, s.count, s.capacity, H / Hkv, Hkv, dkv_stride};
+    a.ragged = RaggedWork{offsets, n, s.items, s.count, s.capacity, H / Hkv, Hkv, s.parts, s.part_heads, s.part_dk, s.part_dv, dkv_stride};
     BwdStatRows ext{nullptr, nullptr, 0.f};
     if (d == 64) {
         ext = BwdStatRows{s.lse_ext, s.d_ext, 1.0f / scale};
@@ -967,9 +978,9 @@ extern "C" int b200attn_bwd_bf16_ragged(const void* q, const void* k, const void
         ScopedKernelTimer timer(1, stream);
         RETURN_IF_CUDA(d == 64 ? launch_attn_bwd_ragged64(a, stream) : launch_attn_bwd_ragged128(a, stream), "packed backward launch");
     }
-    // the head-dim-64 kernel leaves the softmax scale out of dS: dK is scaled where it is stored, dQ here
-    RETURN_IF_CUDA(launch_ragged_dq_convert(s.dq_acc, static_cast<__nv_bfloat16*>(dq), dq_stride, offsets, n, total, H, d,
-                                            d == 64 ? scale : 1.0f, stream), "dq convert");
+    // the head-dim-64 kernel leaves the softmax scale out of dS: dK is scaled where it is stored, dQ here (with parts: there)
+    RETURN_IF_CUDA(launch_ragged_convert(s.dq_acc, static_cast<__nv_bfloat16*>(dq), dq_stride, static_cast<__nv_bfloat16*>(dk),
+                                         static_cast<__nv_bfloat16*>(dv), total, H, d, d == 64 && s.parts == 1 ? scale : 1.0f, a.ragged, stream), "convert");
     return B200ATTN_OK;
 }
 

@@ -149,25 +149,52 @@ __global__ void __launch_bounds__(256) ragged_prepass_kernel(const __nv_bfloat16
     }
 }
 
-__global__ void __launch_bounds__(256) ragged_dq_convert_kernel(const float* __restrict__ acc, __nv_bfloat16* __restrict__ dq,
-                                                                long long dq_stride, const int* __restrict__ offsets, int n, int T, int H,
-                                                                int d, float scale) {
+// Rows in token order: the T x H rows of dq, then (PARTS) the T x kv_heads rows of dk and those of dv.
+template <bool PARTS>
+__global__ void __launch_bounds__(256) ragged_convert_kernel(const float* __restrict__ acc, __nv_bfloat16* __restrict__ dq, long long dq_stride,
+                                                             __nv_bfloat16* __restrict__ dk, __nv_bfloat16* __restrict__ dv, int T, int H, int d,
+                                                             float scale, const RaggedWork w) {
     pdl_launch_dependents();
     pdl_wait();
     const int tpr = d / 8;
     const long long gid = blockIdx.x * 256ll + threadIdx.x;
-    const long long row = gid / tpr;
+    long long row = gid / tpr;
     const int e = int(gid % tpr) * 8;
-    const int t = int(row / H), h = int(row % H);
-    if (row >= (long long)T * H || t < offsets[0] || t >= offsets[n]) return;  // rows of no sequence stay as they are
-    const float4 a0 = __ldg(reinterpret_cast<const float4*>(acc + row * d + e));
-    const float4 a1 = __ldg(reinterpret_cast<const float4*>(acc + row * d + e + 4));
-    uint4 w;
-    w.x = pack_bf16x2(a0.x * scale, a0.y * scale);
-    w.y = pack_bf16x2(a0.z * scale, a0.w * scale);
-    w.z = pack_bf16x2(a1.x * scale, a1.y * scale);
-    w.w = pack_bf16x2(a1.z * scale, a1.w * scale);
-    *reinterpret_cast<uint4*>(dq + t * dq_stride + (long long)h * d + e) = w;
+    auto store = [&](__nv_bfloat16* dst, const float* x, float f) {
+        uint4 y;
+        y.x = pack_bf16x2(x[0] * f, x[1] * f);
+        y.y = pack_bf16x2(x[2] * f, x[3] * f);
+        y.z = pack_bf16x2(x[4] * f, x[5] * f);
+        y.w = pack_bf16x2(x[6] * f, x[7] * f);
+        *reinterpret_cast<uint4*>(dst) = y;
+    };
+    auto in_sequence = [&](int t) { return t >= w.offsets[0] && t < w.offsets[w.n]; };  // other rows stay as they are
+    if (row < (long long)T * H) {
+        const int t = int(row / H), h = int(row % H);
+        if (!in_sequence(t)) return;
+        const float4 a0 = __ldg(reinterpret_cast<const float4*>(acc + row * d + e));
+        const float4 a1 = __ldg(reinterpret_cast<const float4*>(acc + row * d + e + 4));
+        const float x[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
+        store(dq + t * dq_stride + (long long)h * d + e, x, scale);
+        return;
+    }
+    if constexpr (!PARTS) return;
+    const long long rows = (long long)T * w.kv_heads;
+    row -= (long long)T * H;
+    const bool is_dv = row >= rows;
+    if (is_dv) row -= rows;
+    if (row >= rows) return;
+    const int t = int(row / w.kv_heads), h = int(row % w.kv_heads);
+    if (!in_sequence(t)) return;
+    const float* src = (is_dv ? w.part_dv : w.part_dk) + row * d + e;
+    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int p = 0; p < w.parts; ++p) {
+        const float4* from = reinterpret_cast<const float4*>(src + p * rows * d);
+        const float4 a0 = __ldg(from), a1 = __ldg(from + 1);
+        x[0] += a0.x, x[1] += a0.y, x[2] += a0.z, x[3] += a0.w;
+        x[4] += a1.x, x[5] += a1.y, x[6] += a1.z, x[7] += a1.w;
+    }
+    store((is_dv ? dv : dk) + t * w.out_stride + (long long)h * d + e, x, 1.0f);
 }
 
 }  // namespace
@@ -185,12 +212,11 @@ cudaError_t launch_ragged_prepass(const __nv_bfloat16* o, long long o_stride, co
                       dq_acc, T, H, d, ext, w, plan_shift(T));
 }
 
-cudaError_t launch_ragged_dq_convert(const float* dq_acc, __nv_bfloat16* dq, long long dq_stride, const int* offsets, int n, int T,
-                                     int H, int d, float scale, cudaStream_t stream) {
-    const long long blocks = ((long long)T * H * (d / 8) + 255) / 256;
+cudaError_t launch_ragged_convert(const float* dq_acc, __nv_bfloat16* dq, long long dq_stride, __nv_bfloat16* dk, __nv_bfloat16* dv, int T,
+                                  int H, int d, float scale, const RaggedWork& w, cudaStream_t stream) {
+    const long long rows = (long long)T * (H + (w.parts > 1 ? 2 * w.kv_heads : 0)), blocks = (rows * (d / 8) + 255) / 256;
     if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-    return launch_pdl(ragged_dq_convert_kernel, dim3((unsigned int)blocks), dim3(256), 0, stream, dq_acc, dq, dq_stride, offsets, n, T, H,
-                      d, scale);
+    return launch_pdl(w.parts > 1 ? ragged_convert_kernel<true> : ragged_convert_kernel<false>, dim3((unsigned int)blocks), dim3(256), 0, stream, dq_acc, dq, dq_stride, dk, dv, T, H, d, scale, w);
 }
 
 }  // namespace b200attn

@@ -99,6 +99,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc_kernel(const __grid_c
     int bh = 0, jt = 0, hh = 0, bb = 0;  // hh, bb: (key) head and batch coordinates of the 4-D tensor maps
     int n_it = 0;                        // steps: query tiles jt .. n_tiles-1 (RAGGED: of every head of the group)
     int row0 = 0, len = a.T, n_q = 0;    // RAGGED: the sequence's first row and length; query tiles per head
+    int first_head = 0, part = 0;        // RAGGED: first query head of this CTA's part of the group
     if constexpr (!RAGGED) {
         bh = a.tile_major_order ? int(blockIdx.x % a.BH) : int(blockIdx.x / n_tiles);
         jt = a.tile_major_order ? int(blockIdx.x / a.BH) : int(blockIdx.x % n_tiles);
@@ -137,7 +138,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc_kernel(const __grid_c
     // kernel in front of this one in the stream (returns at once for an ordinary launch)
     pdl_wait();
     if constexpr (RAGGED) {
-        const int item = int(blockIdx.x / unsigned(a.ragged.kv_heads));
+        part = int(blockIdx.x / unsigned(a.ragged.kv_heads)) % a.ragged.parts;
+        const int item = int(blockIdx.x / unsigned(a.ragged.kv_heads * a.ragged.parts));
         if (item >= a.ragged.count[0]) {  // the host knows an upper bound only
             __syncthreads();
             if (warp == kProducerWarp) tmem_dealloc(tmem, Cfg::kTmemCols);
@@ -145,12 +147,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc_kernel(const __grid_c
         }
         const int4 w = a.ragged.items[item];
         hh = int(blockIdx.x % unsigned(a.ragged.kv_heads));
-        row0 = w.x, len = w.y, n_q = w.z, jt = (len + kBKV - 1) / kBKV - n_q, n_it = n_q * a.ragged.group;
+        row0 = w.x, len = w.y, n_q = w.z, jt = (len + kBKV - 1) / kBKV - n_q;
+        first_head = hh * a.ragged.group + part * a.ragged.part_heads;
+        n_it = n_q * min(a.ragged.part_heads, a.ragged.group - part * a.ragged.part_heads);
     }
     const int valid_kv = RAGGED ? min(kBKV, len - jt * kBKV) : kBKV;  // keys of this tile that belong to the sequence
     // query tile and head of step `it`, and the tile's rows that belong to the sequence
     auto q_tile = [&](int it) { return RAGGED ? jt + it % n_q : jt + it; };
-    auto q_head = [&](int it) { return RAGGED ? hh * a.ragged.group + it / n_q : hh; };
+    auto q_head = [&](int it) { return RAGGED ? first_head + it / n_q : hh; };
     auto q_valid = [&](int it) { return min(kBQ, len - q_tile(it) * kBQ); };
 
     if (warp == kProducerWarp) {
@@ -477,6 +481,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc_kernel(const __grid_c
                                 make_float4(__uint_as_float(v[x]), __uint_as_float(v[x + 1]), __uint_as_float(v[x + 2]),
                                             __uint_as_float(v[x + 3]));
                     }
+                } else if (RAGGED && a.ragged.parts > 1) {
+                    if (r < valid_kv) {
+                        float* dst = (which == 0 ? a.ragged.part_dv : a.ragged.part_dk) +
+                                     (((long long)part * a.T + row0 + kv_g) * a.ragged.kv_heads + hh) * D + c;
+#pragma unroll
+                        for (int x = 0; x < 32; x += 4)
+                            *reinterpret_cast<float4*>(dst + x) =
+                                make_float4(__uint_as_float(v[x]), __uint_as_float(v[x + 1]), __uint_as_float(v[x + 2]),
+                                            __uint_as_float(v[x + 3]));
+                    }
                 } else {
                     uint8_t* atom = stage + (c >> 6) * kAtomBytes;
 #pragma unroll
@@ -497,7 +511,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc_kernel(const __grid_c
                 }
             }
         }
-        if (!GRADS_F32 && !partial) {
+        if (!GRADS_F32 && !partial && !(RAGGED && a.ragged.parts > 1)) {
             fence_proxy_async_smem();
             named_bar_sync(1, kComputeThreads);
             if (tid == 0) {
@@ -655,7 +669,7 @@ cudaError_t launch_attn_bwd_ragged128(const TcBwdArgs& a, cudaStream_t stream) {
     auto kern = attn_bwd_tc_kernel<128, false, true>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
     if (e != cudaSuccess) return e;
-    const long long blocks = (long long)a.ragged.capacity * a.ragged.kv_heads;
+    const long long blocks = (long long)a.ragged.capacity * a.ragged.kv_heads * a.ragged.parts;
     if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
     return launch_pdl(kern, dim3((unsigned int)blocks), dim3(kThreads), Cfg::kSmemBytes, stream, a);
 }

@@ -100,6 +100,7 @@ struct Cursor {
     int n, g;
     int bh, jt, n_it, it, hh, bb;
     int row0, len, n_q, sub, hq;  // hq: query head of this step (= hh unless RAGGED)
+    int part;                     // RAGGED: part of the group that this item's heads are
     bool valid;
     __device__ __forceinline__ bool first() const { return it == 0; }
     __device__ __forceinline__ bool last() const { return it == n_it - 1; }
@@ -134,6 +135,7 @@ __device__ __forceinline__ uint64_t make_smem_desc_sw32(uint32_t smem_addr) {
     return d;
 }
 
+// RAGGED: packed sequences; with GRADS_F32 the heads of a group are shared out (RaggedWork::parts) and dK / dV are FP32 partial sums.
 template <bool GRADS_F32, bool RAGGED>
 __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc64_kernel(const __grid_constant__ TcBwdArgs a) {
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -223,11 +225,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc64_kernel(const __grid
             c.jt = (c.len + kBKV - 1) / kBKV - c.n_q;
             c.n_it = c.n_q * a.ragged.group;
             c.hq = c.hh * a.ragged.group;
+            if constexpr (GRADS_F32) {
+                c.part = (w / a.ragged.kv_heads) % a.ragged.parts;
+                c.n_it = c.n_q * min(a.ragged.part_heads, a.ragged.group - c.part * a.ragged.part_heads);
+                c.hq += c.part * a.ragged.part_heads;
+            }
         } else if (c.valid) {
             const int4 f = decode_item(w, a.BH, a.H, n_tiles, a.tile_major_order);
             c.bh = f.x, c.jt = f.y, c.hh = f.z, c.bb = f.w;
             c.n_it = c.n_q = n_tiles - c.jt;  // query tiles jt .. n_tiles-1; tiles before the diagonal are skipped
-            c.row0 = 0, c.len = a.T, c.hq = c.hh;
+            c.row0 = 0, c.len = a.T, c.hq = c.hh, c.part = 0;
         }
         c.it = 0;
     };
@@ -270,11 +277,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc64_kernel(const __grid
             tma_prefetch_desc(&a.map_lse_ext);
             tma_prefetch_desc(&a.map_d_ext);
             int published = 0;
-            const int n_items = RAGGED ? a.ragged.count[0] * a.ragged.kv_heads : total_items;
+            const int n_items = RAGGED ? a.ragged.count[0] * a.ragged.kv_heads * a.ragged.parts : total_items;
             auto publish_next = [&]() {
                 int w = int(atomicAdd(a.work_counter, 1u));
                 if (w >= n_items) w = -1;
-                if (RAGGED && w >= 0) s_work[published % kItemRing] = a.ragged.items[w / a.ragged.kv_heads];
+                if (RAGGED && w >= 0) s_work[published % kItemRing] = a.ragged.items[w / (a.ragged.kv_heads * a.ragged.parts)];
                 s_item[published % kItemRing] = w;
                 mbar_arrive(&bars.item_full[published % kItemRing]);  // release: the slot is written before the arrival
                 ++published;
@@ -643,7 +650,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_bwd_tc64_kernel(const __grid
                         const float mul = (which == 1) ? a.scale : 1.0f;  // dK: dS was left unscaled
                         if (in_range) {
                             if constexpr (GRADS_F32) {
-                                float* dst = reinterpret_cast<float*>(which == 0 ? a.dv : a.dk) + ((long long)prev.bh * a.T + kv_g) * kD;
+                                float* dst = RAGGED ? (which == 0 ? a.ragged.part_dv : a.ragged.part_dk) +
+                                                          (((long long)prev.part * a.T + kv_g) * a.ragged.kv_heads + prev.hh) * kD
+                                                    : reinterpret_cast<float*>(which == 0 ? a.dv : a.dk) + ((long long)prev.bh * a.T + kv_g) * kD;
 #pragma unroll
                                 for (int x = 0; x < kD; x += 4)
                                     *reinterpret_cast<float4*>(dst + x) =
@@ -692,18 +701,23 @@ cudaError_t launch_bwd64(const TcBwdArgs& a, cudaStream_t stream) {
     return launch_pdl(kern, dim3((unsigned int)blocks), dim3(kThreads), kSmemBytes, stream, a);
 }
 
-}  // namespace
-
-cudaError_t launch_attn_bwd_ragged64(const TcBwdArgs& a, cudaStream_t stream) {
-    auto kern = attn_bwd_tc64_kernel<false, true>;
+template <bool PARTS>
+cudaError_t launch_bwd_ragged64(const TcBwdArgs& a, cudaStream_t stream) {
+    auto kern = attn_bwd_tc64_kernel<PARTS, true>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
     if (e != cudaSuccess) return e;
     int dev = 0, sms = 0;
     if ((e = cudaGetDevice(&dev)) != cudaSuccess) return e;
     if ((e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
-    const long long items = (long long)a.ragged.capacity * a.ragged.kv_heads;
+    const long long items = (long long)a.ragged.capacity * a.ragged.kv_heads * a.ragged.parts;
     if (items > 0x7fffffffLL) return cudaErrorInvalidValue;
     return launch_pdl(kern, dim3((unsigned int)(items < sms ? items : sms)), dim3(kThreads), kSmemBytes, stream, a);
+}
+
+}  // namespace
+
+cudaError_t launch_attn_bwd_ragged64(const TcBwdArgs& a, cudaStream_t stream) {
+    return a.ragged.parts > 1 ? launch_bwd_ragged64<true>(a, stream) : launch_bwd_ragged64<false>(a, stream);
 }
 
 cudaError_t launch_attn_bwd_tc64(const TcBwdArgs& a, cudaStream_t stream) {

@@ -96,6 +96,10 @@ struct RaggedWork {
     int capacity;         // upper bound of the number of items, known to the host
     int group;            // query heads per key head
     int kv_heads;
+    int parts;            // backward: the heads of a group go to so many CTAs (1: to one, which sums dK and dV of the group)
+    int part_heads;       // query heads per part: group / parts, rounded up (the last part may have fewer)
+    float* part_dk;       // parts > 1: FP32 (parts, T, kv_heads, d) sums, joined by launch_ragged_convert
+    float* part_dv;
     long long out_stride; // element stride between rows of `out` (forward) or of dk and dv (backward)
 };
 constexpr int kRaggedFindMax = 128;
@@ -183,9 +187,10 @@ cudaError_t launch_dq_convert(const float* dq_acc, __nv_bfloat16* dq, long long 
 cudaError_t launch_ragged_prepass(const __nv_bfloat16* o, long long o_stride, const __nv_bfloat16* dO, long long do_stride,
                                   const float* lse, float* D, float* lse2, float* dq_acc, int T, int H, int d, BwdStatRows ext,
                                   const RaggedWork& w, cudaStream_t stream);
-// dq (BF16 rows at dq_stride) = dq_acc * scale for the rows offsets[0] .. offsets[n] (clipped to [0, T]); others keep their values.
-cudaError_t launch_ragged_dq_convert(const float* dq_acc, __nv_bfloat16* dq, long long dq_stride, const int* offsets, int n, int T,
-                                     int H, int d, float scale, cudaStream_t stream);
+// dq (BF16 rows at dq_stride) = dq_acc * scale and, with parts > 1, dk and dv (rows at w.out_stride) = the sums of their parts, for the
+// rows offsets[0] .. offsets[n]; others keep their values.
+cudaError_t launch_ragged_convert(const float* dq_acc, __nv_bfloat16* dq, long long dq_stride, __nv_bfloat16* dk, __nv_bfloat16* dv, int T,
+                                  int H, int d, float scale, const RaggedWork& w, cudaStream_t stream);
 
 // ------------------------------------------------------------------ attn_decode.cu (one query token per sequence)
 struct DecodeArgs {

@@ -54,7 +54,7 @@ _SIGNATURES = {
     "b200attn_bwd_bf16_noalloc": ([_P] * 9 + [_I, _I, _I, _F, _P], _I),
     "b200attn_fwd_bf16_packed": ([_P] * 3 + [_I, _I, _I, _I, _F, _P], _I),
     "b200attn_bwd_bf16_packed": ([_P] * 5 + [_I, _I, _I, _I, _F, _P], _I),
-    "b200attn_ragged_workspace_bytes": ([_I] * 5, _LL),
+    "b200attn_ragged_workspace_bytes": ([_I] * 6, _LL),
     "b200attn_fwd_bf16_ragged": ([_P] * 7 + [_LL] + [_I] * 5 + [_LL] * 3 + [_F, _P], _I),
     "b200attn_bwd_bf16_ragged": ([_P] * 11 + [_LL] + [_I] * 5 + [_LL] * 6 + [_F, _P], _I),
     "b200attn_decode_workspace_bytes": ([_I] * 5, _LL),
