@@ -115,6 +115,11 @@ __global__ void __launch_bounds__(kThreads, 2) attn_fwd_tc_short_kernel(const __
         mbar_fence_init();
     }
     if (warp == 4) {
+        if (RAGGED && lane == 0) {  // under the set-up
+            tma_prefetch_desc(&a.map_q);
+            tma_prefetch_desc(&a.map_k);
+            tma_prefetch_desc(&a.map_v);
+        }
         tmem_alloc(&tmem_base_slot, Cfg::kTmemCols);
         tmem_relinquish();
     }
@@ -127,10 +132,16 @@ __global__ void __launch_bounds__(kThreads, 2) attn_fwd_tc_short_kernel(const __
     pdl_wait();
     if constexpr (RAGGED) {  // the heads of one tile are neighbours: those of a group read the same key tiles
         const int item = int(blockIdx.x / unsigned(a.H));
-        int4 w = make_int4(0, 0, 0, 0);
-        if (a.ragged.items == nullptr) w = ragged_find(a.ragged.offsets, a.ragged.n, a.T, item, lane);
-        else if (item < a.ragged.count[0]) w = a.ragged.items[item];
-        if (w.z == 0) {  // the host knows an upper bound only
+        int4 w;
+        bool none;
+        if (a.ragged.items == nullptr) {
+            w = ragged_find(a.ragged.offsets, a.ragged.n, a.T, item, lane);
+            none = w.z == 0;
+        } else {  // both loads under way together: the list has room for every item of the grid
+            w = a.ragged.items[item];
+            none = item >= a.ragged.count[0];
+        }
+        if (none) {  // the host knows an upper bound only
             __syncthreads();
             if (warp == 4) tmem_dealloc(tmem, Cfg::kTmemCols);
             return;
@@ -143,9 +154,11 @@ __global__ void __launch_bounds__(kThreads, 2) attn_fwd_tc_short_kernel(const __
     if (warp == 4) {
         // ------------------------------------------------------------ TMA producer
         if (lane == 0) {
-            tma_prefetch_desc(&a.map_q);
-            tma_prefetch_desc(&a.map_k);
-            tma_prefetch_desc(&a.map_v);
+            if (!RAGGED) {
+                tma_prefetch_desc(&a.map_q);
+                tma_prefetch_desc(&a.map_k);
+                tma_prefetch_desc(&a.map_v);
+            }
             mbar_expect_tx(&bars.q_full, Cfg::kTileBytes);
             for (int at = 0; at < Cfg::kAtoms; ++at)
                 tma_load_4d(sQ + at * kAtomBytes, &a.map_q, &bars.q_full, at * 64, row0 + qt * kBM, hh, bb);
