@@ -8,7 +8,7 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
-#include <ATen/ops/empty.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <ATen/ops/zeros.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -111,7 +111,9 @@ void need_args(Py_ssize_t n, Py_ssize_t want) {
         throw PyFailed{};
     }
 }
-at::Tensor empty(c10::IntArrayRef sizes, at::ScalarType type, at::Device device) { return at::empty(sizes, at::TensorOptions(type).device(device)); }
+at::Tensor empty(c10::IntArrayRef sizes, at::ScalarType type, at::Device device) {
+    return at::Tensor(at::detail::empty_cuda(sizes, type, device, std::nullopt));  // torch.empty without its dispatch
+}
 at::Tensor zeros(c10::IntArrayRef sizes, at::ScalarType type, at::Device device) { return at::zeros(sizes, at::TensorOptions(type).device(device)); }
 // Scratch of one call from torch's allocator: ordered with the stream, its own in every captured graph.
 at::Tensor scratch(int64_t bytes, at::Device device) { return empty({bytes > 16 ? bytes : 16}, at::kByte, device); }

@@ -16,8 +16,11 @@
 //
 // A CTA of four warps takes one split of one (sequence, key head); warp w takes the 16-key tiles w, w + 4, ... of it with its
 // own running maximum and sum, and the warps meet in shared memory. The splits of a sequence are equal parts of ITS length
-// (read on the device), so a long capacity with short lengths costs nothing. With more than one split the parts go to a
-// workspace and a second kernel joins them in a fixed order: results do not depend on timing.
+// (read on the device), so a long capacity with short lengths costs nothing. Up to eight splits are a cluster and join through
+// distributed shared memory; more of them go to a workspace, which a second kernel joins. Either adds in a fixed order: results do
+// not depend on timing.
+#include <cooperative_groups.h>
+
 #include "kernels.cuh"
 #include "tc_common.cuh"
 
@@ -29,6 +32,7 @@ constexpr int kThreads = 32 * kWarps;
 constexpr int kTile = 16;                      // keys per warp and step
 constexpr int kStages = 3;                     // steps of K and V in flight per warp
 constexpr int kRound = kTile * kWarps;         // keys of a CTA and step; a split is a multiple of it
+constexpr int kMaxCluster = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kNoKey = -1e30f;               // running maximum before the first key (finite: differences of it are numbers)
@@ -56,8 +60,14 @@ __device__ __forceinline__ int chunk_of(int len, int splits) {
 }
 __device__ __forceinline__ int length_of(const DecodeArgs& a, int b) { return min(max(a.lengths[b], 0), a.T); }
 
-// R = 8: the block of heads has at most 8; R = 16: up to 16.
-template <int D, int R>
+__device__ __forceinline__ void write_out(const DecodeArgs& a, int b, int h, int D, int e, float M, float L, float x0, float x1) {
+    const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);  // no keys: zeros; NaN stays NaN
+    *reinterpret_cast<uint32_t*>(a.out + ((long long)b * a.H + h) * D + e) = pack_bf16x2(x0 * inv, x1 * inv);
+    if (e == 0) a.lse[(long long)b * a.H + h] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
+}
+
+// R = 8: the block of heads has at most 8; R = 16: up to 16. CLUSTER: the splits of a sequence are the CTAs of a cluster.
+template <int D, int R, bool CLUSTER>
 __global__ void __launch_bounds__(kThreads, 2) attn_decode_kernel(const DecodeArgs a) {
     constexpr int kRowsPerLane = R / 8;  // head g, and head g + 8
     constexpr int kSets = D / 32;        // 16-byte pieces of a key per lane
@@ -65,6 +75,8 @@ __global__ void __launch_bounds__(kThreads, 2) attn_decode_kernel(const DecodeAr
     extern __shared__ __align__(16) float s_sums[];
     float (*s_o)[R][D] = reinterpret_cast<float (*)[R][D]>(s_sums);  // [warp][head][dim]
     __shared__ float s_m[kWarps][R], s_l[kWarps][R];
+    __shared__ float2 s_ml[CLUSTER ? R : 1];                              // this CTA's maximum and sum per head
+    float2 (*s_part)[D / 2] = reinterpret_cast<float2 (*)[D / 2]>(s_sums + kWarps * R * D);  // and its output sums, [head][dim pair]
 
     pdl_launch_dependents();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -76,7 +88,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_decode_kernel(const DecodeAr
     const int len = length_of(a, b);
     const int chunk = chunk_of(len, a.splits);
     const int begin = split * chunk, end = min(len, begin + chunk);
-    if (begin >= end && !(split == 0 && a.splits == 1)) return;  // an empty split is never joined
+    if (!CLUSTER && begin >= end && a.splits > 1) return;  // an empty split is never joined
 
     uint32_t qf[kSets][2][4];  // A fragments of the two steps of every set
 #pragma unroll
@@ -255,15 +267,40 @@ __global__ void __launch_bounds__(kThreads, 2) attn_decode_kernel(const DecodeAr
             x0 = fmaf(s_o[w][row][e], f, x0), x1 = fmaf(s_o[w][row][e + 1], f, x1);
         }
         const int h = h0 + row;
-        if (a.splits == 1) {
-            const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);  // no keys: zeros; NaN stays NaN
-            *reinterpret_cast<uint32_t*>(a.out + ((long long)b * a.H + h) * D + e) = pack_bf16x2(x0 * inv, x1 * inv);
-            if (e == 0) a.lse[(long long)b * a.H + h] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
+        if constexpr (CLUSTER) {
+            s_part[row][e / 2] = make_float2(x0, x1);
+            if (e == 0) s_ml[row] = make_float2(M, L);
+        } else if (a.splits == 1) {
+            write_out(a, b, h, D, e, M, L, x0, x1);
         } else {
             const long long part = ((long long)b * a.H + h) * a.splits + split;
             *reinterpret_cast<float2*>(a.part_o + part * D + e) = make_float2(x0, x1);
             if (e == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * part) = make_float2(M, L);
         }
+    }
+    if constexpr (CLUSTER) {  // every CTA joins its share of the outputs
+        cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+        cluster.sync();
+        for (int i = split * kThreads + tid; i < rows * (D / 2); i += a.splits * kThreads) {
+            const int row = i / (D / 2), e = i % (D / 2);
+            float2 ml[kMaxCluster], x[kMaxCluster];
+            float M = kNoKey, L = 0.f, x0 = 0.f, x1 = 0.f;
+#pragma unroll
+            for (int p = 0; p < kMaxCluster; ++p) {
+                if (p >= a.splits) break;
+                ml[p] = *cluster.map_shared_rank(&s_ml[row], p);
+                x[p] = *cluster.map_shared_rank(&s_part[row][e], p);
+                M = fmaxf(M, ml[p].x);
+            }
+#pragma unroll
+            for (int p = 0; p < kMaxCluster; ++p) {
+                if (p >= a.splits) break;
+                const float f = fast_exp2(ml[p].x - M);
+                L = fmaf(ml[p].y, f, L), x0 = fmaf(x[p].x, f, x0), x1 = fmaf(x[p].y, f, x1);
+            }
+            write_out(a, b, h0 + row, D, 2 * e, M, L, x0, x1);
+        }
+        cluster.sync();  // the others have read this CTA's shared memory
     }
 }
 
@@ -312,25 +349,28 @@ __global__ void __launch_bounds__(kJoinThreads) attn_decode_join_kernel(const De
     if (grp == 0) {
 #pragma unroll
         for (int i = 1; i < kGroups; ++i) x0 += s_x[i][e].x, x1 += s_x[i][e].y;
-        const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);
-        *reinterpret_cast<uint32_t*>(a.out + ((long long)b * a.H + h) * D + 2 * e) = pack_bf16x2(x0 * inv, x1 * inv);
-        if (e == 0) a.lse[(long long)b * a.H + h] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
+        write_out(a, b, h, D, 2 * e, M, L, x0, x1);
     }
 }
 
 template <int D, int R>
 cudaError_t launch(const DecodeArgs& a, cudaStream_t stream) {
-    constexpr int stages = kWarps * kStages * kTile * D * 2 * 2, sums = kWarps * R * D * int(sizeof(float));
+    constexpr int stages = kWarps * kStages * kTile * D * 2 * 2, sums = (kWarps + 1) * R * D * int(sizeof(float));
     constexpr int smem = stages > sums ? stages : sums;
-    cudaError_t e = cudaFuncSetAttribute(attn_decode_kernel<D, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const bool cluster = a.splits > 1 && a.splits <= kMaxCluster;
+    auto kern = cluster ? attn_decode_kernel<D, R, true> : attn_decode_kernel<D, R, false>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
-    e = launch_pdl(attn_decode_kernel<D, R>, dim3(a.Hkv * a.head_blocks, a.splits, a.B), dim3(kThreads), smem, stream, a);
-    if (e != cudaSuccess || a.splits == 1) return e;
+    const dim3 grid(a.Hkv * a.head_blocks, a.splits, a.B);
+    e = cluster ? launch_pdl_cluster(kern, grid, dim3(1, a.splits, 1), dim3(kThreads), smem, stream, a)
+                : launch_pdl(kern, grid, dim3(kThreads), smem, stream, a);
+    if (e != cudaSuccess || a.splits == 1 || cluster) return e;
     return launch_pdl(attn_decode_join_kernel<D>, dim3(a.H, a.B), dim3(kJoinThreads), 0, stream, a);
 }
 
 }  // namespace
 
+bool decode_needs_workspace(int splits) { return splits > kMaxCluster; }
 int decode_splits(int B, int T, int H, int Hkv) {
     const int G = H / Hkv, R = G <= 8 ? 8 : 16;
     const long long items = (long long)B * Hkv * ((G + R - 1) / R);

@@ -29,6 +29,26 @@ cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t sme
     return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
 }
 
+// The same with clusters of `cluster` CTAs.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_pdl_cluster(void (*kern)(KArgs...), dim3 grid, dim3 cluster, dim3 block, size_t smem, cudaStream_t stream, Args&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster.x;
+    attr[1].val.clusterDim.y = cluster.y;
+    attr[1].val.clusterDim.z = cluster.z;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+}
+
 // ------------------------------------------------------------------ layout_kernels.cu
 // TOut is float or __nv_bfloat16 for the split, TIn likewise for the merges.
 template <typename TOut>
@@ -198,7 +218,7 @@ struct DecodeArgs {
     const int* lengths;
     __nv_bfloat16* out;             // (B, H, d)
     float* lse;                     // (B, H)
-    float* part_o;                  // splits > 1: (B, H, splits, d) sums and (B, H, splits, 2) maximum and sum
+    float* part_o;                  // decode_needs_workspace(splits): (B, H, splits, d) sums and (B, H, splits, 2) maximum and sum
     float* part_ml;
     int B, T, H, Hkv, d;
     long long q_stride;             // elements from sequence to sequence
@@ -208,6 +228,7 @@ struct DecodeArgs {
     int G, head_blocks;             // filled in by the launcher
 };
 int decode_splits(int B, int T, int H, int Hkv);
+bool decode_needs_workspace(int splits);  // fewer splits join inside a cluster
 cudaError_t launch_attn_decode(DecodeArgs a, cudaStream_t stream);
 
 // ------------------------------------------------------------------ wait_selftest.cu
