@@ -91,7 +91,7 @@ def build(verbose=False, force=False, ptxas_info=False):
         subprocess.check_call(["ar", "rcs", GEMM_AR] + gemm_objs)
     # the loss drop-in (fused softmax cross-entropy) and the token log-probabilities: their own shared + static library, no dependency on the attention engine
     loss_objs = []
-    loss_hdrs = [os.path.join(CSRC, "tc_common.cuh"), os.path.join(HERE, "loss", "loss_internal.h"),
+    loss_hdrs = [os.path.join(CSRC, "tc_common.cuh"), os.path.join(CSRC, "kernels.cuh"), os.path.join(HERE, "loss", "loss_internal.h"),
                  os.path.join(HERE, "..", "include", "kernels", "loss.cuh"), os.path.join(HERE, "..", "include", "b200loss.h")]
     for name in ("cross_entropy", "token_logprobs"):
         src = os.path.join(HERE, "loss", name + ".cu")

@@ -22,11 +22,18 @@
 #include <stdint.h>
 
 #include "b200loss.h"
+#include "kernels.cuh"
 #include "loss_internal.h"
+#include "tc_common.cuh"
 
 namespace cg = cooperative_groups;
 
 namespace {
+
+using b200attn::launch_pdl;
+using b200attn::launch_pdl_cluster;
+using b200attn::pdl_launch_dependents;
+using b200attn::pdl_wait;
 
 constexpr int kWarpRowThreads = 256; // CTAs of the kernels that give a row to a warp
 constexpr int kUnroll = 4;           // 16-byte loads in flight per thread
@@ -250,13 +257,11 @@ struct FwdArgs {
 __device__ __forceinline__ float logprob_of(float x, const RowStat& a, float inv_temperature) {
     return a.m == -INFINITY ? -INFINITY : fmaf(x - a.m, inv_temperature, -a.ln_s);
 }
-template <typename T>
-__device__ __forceinline__ void write_row(const FwdArgs& a, const T* row, int r, const RowStat& st) {
-    const int target = a.targets[r];
+__device__ __forceinline__ void write_row(const FwdArgs& a, int r, const RowStat& st, bool given, float target_x) {
     a.stats[2ll * r] = st.m;
     a.stats[2ll * r + 1] = st.ln_s;
     a.entropy[r] = st.entropy;
-    a.logprobs[r] = (unsigned)target < (unsigned)a.V ? logprob_of(Elem<T>::load(row + target), st, a.inv_temperature) : 0.f;
+    a.logprobs[r] = given ? logprob_of(target_x, st, a.inv_temperature) : 0.f;
 }
 
 // ---------------------------------------------------------------- forward, one CTA (or one cluster of CTAs) per row
@@ -297,30 +302,24 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const FwdArgs 
     __shared__ int s_nhot, s_ncand;
     __shared__ uint32_t s_threshold;
 
+    pdl_launch_dependents();
     const cg::cluster_group cluster = cg::this_cluster();
     const int parts = int(cluster.num_blocks()), part = int(cluster.block_rank());
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const float c = a.inv_temperature * kLog2e;
+    const Pair c2 = pair(c, c);
+    const uint4 nothing = make_uint4(Elem<T>::kNegInf, Elem<T>::kNegInf, Elem<T>::kNegInf, Elem<T>::kNegInf);
+
     const int r = int(blockIdx.x / unsigned(parts));
     const T* row = static_cast<const T*>(a.logits) + a.row_stride * r;
     const RowSplit sp = split_row(row, a.V);
-    const uint4* vec = reinterpret_cast<const uint4*>(row + sp.head);
+    const int head = sp.head;
+    const uint4* vec = reinterpret_cast<const uint4*>(row + head);
     const int begin = int((long long)sp.vecs * part / parts), end = int((long long)sp.vecs * (part + 1) / parts);
-    const float c = a.inv_temperature * kLog2e;
-
     // the single element in front of or behind the vectors that this thread owns, if any
     const int edge = (part == 0 && tid < sp.head) ? tid
                      : (part == parts - 1 && tid >= 32 && tid < 32 + sp.tail) ? sp.head + sp.vecs * E + (tid - 32)
                                                                               : -1;
-    Stat st{kFloor, 0.f, 0.f};
-    float my_max = -INFINITY;  // of the logits as they are: what the alternatives are found by, and whether the row is wild
-    if (edge >= 0) {
-        my_max = Elem<T>::load(row + edge);
-        st.m = max_nan(my_max, kFloor);
-        st.s = 1.f;
-    }
-    Pair s2 = pair(st.s, 0.f), t2 = pair(0.f, 0.f);
-    const Pair c2 = pair(c, c);
-    const uint4 nothing = make_uint4(Elem<T>::kNegInf, Elem<T>::kNegInf, Elem<T>::kNegInf, Elem<T>::kNegInf);
     uint4 next[kUnroll];  // the next round's loads are under way while this one is added
     auto load_round = [&](int i0) {
 #pragma unroll
@@ -329,7 +328,15 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const FwdArgs 
             next[u] = i < end ? __ldg(vec + i) : nothing;
         }
     };
+    pdl_wait();
     load_round(begin);
+    // needed at the end only: under way with the first round
+    const float edge_x = edge >= 0 ? Elem<T>::load(row + edge) : -INFINITY;
+    const int target = a.targets[r];
+    const bool given = (unsigned)target < (unsigned)a.V;
+    Stat st{kFloor, 0.f, 0.f};
+    float my_max = edge_x;  // of the logits as they are: what the alternatives are found by, and whether the row is wild
+    Pair s2 = pair(0.f, 0.f), t2 = pair(0.f, 0.f);
     // The row's rounds in at most kSegments segments: a thread's maximum is kept for each (alternatives only).
     const int rounds = (end - begin + kThreads * kUnroll - 1) / (kThreads * kUnroll), per_segment = max(1, (rounds + kSegments - 1) / kSegments);
     float segment_max = -INFINITY;
@@ -348,7 +355,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const FwdArgs 
                 segment_max = -INFINITY, left = per_segment;
             }
         }
-        const float m = max_nan(st.m, my_max);
+        const float m = max_nan(st.m, round_max);
         if (m != st.m) {  // a new maximum, or NaN
             float sa, sb, ta, tb;
             split(s2, sa, sb), split(t2, ta, tb);
@@ -358,11 +365,9 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const FwdArgs 
             s2 = pair(old.s, 0.f), t2 = pair(old.t, 0.f);
         }
         const Pair neg_m = pair(-st.m, -st.m);
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            if (i0 + u * kThreads + warp * 32 >= end) break;  // the last round's rest: nothing for this warp
+        auto add_vec = [&](const uint4& v) {
             float x[E];
-            Elem<T>::unpack(Elem<T>::raise(w[u]), x);
+            Elem<T>::unpack(Elem<T>::raise(v), x);
 #pragma unroll
             for (int e = 0; e < E; e += 2) {
                 float a0, a1;
@@ -372,8 +377,17 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const FwdArgs 
                 s2 = add(s2, ex);
                 t2 = fma(ex, arg, t2);
             }
+        };
+        if (i0 + kThreads * kUnroll <= end) {
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) add_vec(w[u]);
+        } else {  // the last round: not what this warp has nothing of
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u)
+                if (i0 + u * kThreads + warp * 32 < end) add_vec(w[u]);
         }
     }
+    const float target_x = given && tid == 0 ? Elem<T>::load(row + target) : 0.f;  // under way with the reductions
     {
         float sa, sb, ta, tb;
         split(s2, sa, sb), split(t2, ta, tb);
@@ -388,6 +402,10 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const FwdArgs 
 #pragma unroll
     for (int w = 1; w < kWarps; ++w) part_max = max_nan(part_max, s_max[w]);
     rebase(st, max_nan(part_max, kFloor), c);
+    if (edge >= 0) {
+        const float x = (max_nan(edge_x, kFloor) - st.m) * c, e = ex2(x);
+        st.s += e, st.t = fmaf(e, x, st.t);
+    }
     const float warp_s = warp_add(st.s), warp_t = warp_add(st.t);
     if (lane == 0) s_sum[warp] = warp_s, s_sum_a[warp] = warp_t;
     if (a.top > 0 && warp == kWarps - 1) {
@@ -444,10 +462,10 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const FwdArgs 
                 float x[E];
                 Elem<T>::unpack(w[u], x);
 #pragma unroll
-                for (int e = 0; e < E; ++e) consider(x[e], sp.head + at[u] * E + e);
+                for (int e = 0; e < E; ++e) consider(x[e], head + at[u] * E + e);
             }
         }
-        if (edge >= 0) consider(Elem<T>::load(row + edge), edge);
+        if (edge >= 0) consider(edge_x, edge);
         __syncthreads();
         const int n = s_ncand;
         if (n >= a.top && n <= kMaxCand && nhot <= kMaxHot) {
@@ -467,12 +485,12 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const FwdArgs 
                     Elem<T>::unpack(__ldg(vec + i), x);
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
-                        const uint64_t y = candidate(to_key(x[e]), sp.head + i * E + e);
+                        const uint64_t y = candidate(to_key(x[e]), head + i * E + e);
                         if (y < before && y > best) best = y;
                     }
                 }
                 if (edge >= 0) {
-                    const uint64_t y = candidate(to_key(Elem<T>::load(row + edge)), edge);
+                    const uint64_t y = candidate(to_key(edge_x), edge);
                     if (y < before && y > best) best = y;
                 }
 #pragma unroll
@@ -506,7 +524,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const FwdArgs 
 #pragma unroll
                 for (int e = 0; e < E; ++e) add_exact(x[e], row_max, c, s, t);
             }
-            if (edge >= 0) add_exact(Elem<T>::load(row + edge), row_max, c, s, t);
+            if (edge >= 0) add_exact(edge_x, row_max, c, s, t);
         }
         s = warp_add(s), t = warp_add(t);
         __syncthreads();  // s_sum has been read
@@ -545,7 +563,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const FwdArgs 
     }
     __syncthreads();
     const RowStat total = finish(s_total);
-    if (tid == 0) write_row(a, row, r, total);
+    if (tid == 0) write_row(a, r, total, given, target_x);
     if (tid < a.top) {
         const uint64_t y = s_sel[tid];
         a.top_logprobs[(long long)r * a.top + tid] = logprob_of(from_key(uint32_t(y >> 32)), total, a.inv_temperature);
@@ -554,26 +572,37 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const FwdArgs 
 }
 
 // ---------------------------------------------------------------- forward, one warp per (short) row
-template <typename T>
+// N: elements per lane, all of them in registers.
+template <typename T, int N>
 __global__ void __launch_bounds__(kWarpRowThreads) token_logprobs_warp_kernel(const FwdArgs a) {
     constexpr int kWarps = kWarpRowThreads / 32, kList = 128;
     __shared__ uint64_t s_cand[kWarps][kList];
     __shared__ int s_ncand[kWarps];
+    pdl_launch_dependents();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const long long r64 = (long long)blockIdx.x * kWarps + warp;
+    pdl_wait();
     if (r64 >= a.rows) return;
     const int r = int(r64);
     const T* row = static_cast<const T*>(a.logits) + a.row_stride * r;
     const float c = a.inv_temperature * kLog2e;
-    float mine = -INFINITY;
-    for (int v = lane; v < a.V; v += 32) mine = max_nan(mine, Elem<T>::load(row + v));
+    const int target = a.targets[r];
+    float x[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = i * 32 + lane < a.V ? Elem<T>::load(row + i * 32 + lane) : -INFINITY;
+    const bool given = (unsigned)target < (unsigned)a.V;
+    const float target_x = given ? Elem<T>::load(row + target) : 0.f;
+    float mine = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) mine = max_nan(mine, x[i]);
     Stat st{warp_max_nan(mine), 0.f, 0.f};
     if (st.m != -INFINITY) {
-        for (int v = lane; v < a.V; v += 32) add_exact(Elem<T>::load(row + v), st.m, c, st.s, st.t);
+#pragma unroll
+        for (int i = 0; i < N; ++i) add_exact(x[i], st.m, c, st.s, st.t);
         st.s = warp_add(st.s), st.t = warp_add(st.t);
     }
     const RowStat total = finish(st);
-    if (lane == 0) write_row(a, row, r, total);
+    if (lane == 0) write_row(a, r, total, given, target_x);
     if (a.top == 0) return;
 
     // alternatives: as above, with the lane maxima; rows too short for 32 lanes have threshold 0 (every logit is a candidate)
@@ -581,9 +610,11 @@ __global__ void __launch_bounds__(kWarpRowThreads) token_logprobs_warp_kernel(co
     const uint32_t threshold = threshold_of(k, a.top);
     if (lane == 0) s_ncand[warp] = 0;
     __syncwarp();
-    for (int v = lane; v < a.V; v += 32) {
-        const uint32_t key = to_key(Elem<T>::load(row + v));
-        if (key >= threshold) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int v = i * 32 + lane;
+        const uint32_t key = to_key(x[i]);
+        if (v < a.V && key >= threshold) {
             const int at = atomicAdd(&s_ncand[warp], 1);
             if (at < kList) s_cand[warp][at] = candidate(key, v);
         }
@@ -606,9 +637,10 @@ __global__ void __launch_bounds__(kWarpRowThreads) token_logprobs_warp_kernel(co
     uint64_t before = ~uint64_t(0);
     for (int i = 0; i < a.top; ++i) {
         uint64_t best = 0;
-        for (int v = lane; v < a.V; v += 32) {
-            const uint64_t y = candidate(to_key(Elem<T>::load(row + v)), v);
-            if (y < before && y > best) best = y;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const uint64_t y = candidate(to_key(x[j]), j * 32 + lane);
+            if (j * 32 + lane < a.V && y < before && y > best) best = y;
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
@@ -715,15 +747,29 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_bwd_kernel(const BwdA
 template <typename T>
 __global__ void __launch_bounds__(kWarpRowThreads) token_logprobs_bwd_warp_kernel(const BwdArgs a) {
     constexpr int kWarps = kWarpRowThreads / 32;
+    pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
     const long long r64 = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
+    pdl_wait();
     if (r64 >= a.rows) return;
     const int r = int(r64);
     const T* row = static_cast<const T*>(a.logits) + a.row_stride * r;
     T* out = static_cast<T*>(a.dlogits) + a.d_row_stride * r;
     const RowGrad q = row_grad(a, r);
     const float c = a.inv_temperature * kLog2e;
-    for (int v = lane; v < a.V; v += 32) Elem<T>::store(out + v, q.zero ? 0.f : grad_of(q, Elem<T>::load(row + v), c) + (v == q.target ? q.g : 0.f));
+    for (int v0 = 0; v0 < a.V; v0 += 32 * kUnroll) {  // read together, then written: the gradient may go where the logits are
+        float x[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const int v = v0 + u * 32 + lane;
+            x[u] = v < a.V && !q.zero ? Elem<T>::load(row + v) : 0.f;
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const int v = v0 + u * 32 + lane;
+            if (v < a.V) Elem<T>::store(out + v, q.zero ? 0.f : grad_of(q, x[u], c) + (v == q.target ? q.g : 0.f));
+        }
+    }
 }
 
 // ---------------------------------------------------------------- host side
@@ -753,26 +799,15 @@ cudaError_t launch_rows(const FwdArgs& a, cudaStream_t stream) {
     // full round of loads.
     int parts = 1;
     while (parts < kMaxCluster && (long long)a.rows * parts * 2 <= 296 && a.V / (parts * 2) >= kThreads * Elem<T>::kPerVec) parts *= 2;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(a.rows) * unsigned(parts));
-    cfg.blockDim = dim3(kThreads);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = unsigned(parts);
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, kThreads>, a);
+    return launch_pdl_cluster(token_logprobs_kernel<T, kThreads>, dim3(unsigned(a.rows) * unsigned(parts)), dim3(unsigned(parts)), dim3(kThreads), 0, stream, a);
 }
 
 template <typename T>
 cudaError_t launch_forward(const FwdArgs& a, cudaStream_t stream) {
     if (a.V <= kWarpRowVocab) {
         constexpr int rows = kWarpRowThreads / 32;
-        token_logprobs_warp_kernel<T><<<(a.rows + rows - 1) / rows, kWarpRowThreads, 0, stream>>>(a);
-        return cudaGetLastError();
+        auto kern = a.V <= 128 ? token_logprobs_warp_kernel<T, 4> : a.V <= 384 ? token_logprobs_warp_kernel<T, 12> : token_logprobs_warp_kernel<T, 32>;
+        return launch_pdl(kern, dim3((a.rows + rows - 1) / rows), dim3(kWarpRowThreads), 0, stream, a);
     }
     // a thread should have some vectors of its row: short rows get small CTAs
     return a.V <= kSmallRowVecs * Elem<T>::kPerVec ? launch_rows<T, 64>(a, stream) : launch_rows<T, 256>(a, stream);
@@ -783,6 +818,7 @@ cudaError_t launch_gradient(BwdArgs a, cudaStream_t stream) {
     constexpr int per_cta = kThreads * kUnroll * Elem<T>::kPerVec;
     a.chunks = (a.V + per_cta - 1) / per_cta;
     if ((long long)a.rows * a.chunks > 0x7fffffffLL) return cudaErrorInvalidValue;
+    // launched the ordinary way: its many short CTAs pay more for the dependency wait than the overlap gives (8192 x 3000: 21 us, 17 so)
     token_logprobs_bwd_kernel<T, kThreads><<<unsigned(a.rows) * unsigned(a.chunks), kThreads, 0, stream>>>(a);
     return cudaGetLastError();
 }
@@ -793,8 +829,7 @@ cudaError_t launch_backward(const BwdArgs& a, cudaStream_t stream) {
     const bool same_phase = ((x ^ d) & 15u) == 0 && ((a.row_stride - a.d_row_stride) * (long long)sizeof(T)) % 16 == 0;
     if (a.V <= kWarpGradVocab || !same_phase) {
         constexpr int rows = kWarpRowThreads / 32;
-        token_logprobs_bwd_warp_kernel<T><<<(a.rows + rows - 1) / rows, kWarpRowThreads, 0, stream>>>(a);
-        return cudaGetLastError();
+        return launch_pdl(token_logprobs_bwd_warp_kernel<T>, dim3((a.rows + rows - 1) / rows), dim3(kWarpRowThreads), 0, stream, a);
     }
     return a.V <= kSmallRowVecs * Elem<T>::kPerVec ? launch_gradient<T, 64>(a, stream) : launch_gradient<T, 256>(a, stream);
 }
