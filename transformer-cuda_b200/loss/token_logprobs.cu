@@ -38,13 +38,12 @@ using b200attn::pdl_wait;
 constexpr int kWarpRowThreads = 256; // CTAs of the kernels that give a row to a warp
 constexpr int kUnroll = 4;           // 16-byte loads in flight per thread
 constexpr int kMaxTop = 32;
-constexpr int kMaxCand = 1024;
 constexpr int kSegments = 8;
-constexpr int kMaxHot = 256;
 constexpr int kMaxCluster = 8;
 constexpr int kWarpRowVocab = 1024;  // rows up to here are handled by one warp each
 constexpr int kWarpGradVocab = 256;  // the same in the gradient
-constexpr int kSmallRowVecs = 1024;  // rows of up to so many 16-byte vectors by CTAs of 64 threads, longer ones by 256
+constexpr int kSmallRowVecs = 1024;  // rows of up to so many 16-byte vectors by CTAs of 64 threads
+constexpr int kMiddleRowVecs = 8192; // up to here by 128 threads, longer ones by 256
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -1e30f;    // x - m is held above this, so that a masked logit contributes 0 * finite
@@ -290,7 +289,7 @@ __device__ __forceinline__ uint32_t threshold_of(const uint32_t (&k)[N], int top
 
 template <typename T, int kThreads>
 __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const FwdArgs a) {
-    constexpr int E = Elem<T>::kPerVec, kWarps = kThreads / 32;
+    constexpr int E = Elem<T>::kPerVec, kWarps = kThreads / 32, kMaxCand = kThreads >= 256 ? 1024 : 256, kMaxHot = kThreads >= 256 ? 256 : 128;
     __shared__ float s_max[kWarps], s_sum[kWarps], s_sum_a[kWarps], s_part_max;
     __shared__ Stat s_part, s_total;  // of this CTA's part of the row, and of the row
     __shared__ uint32_t s_key[kThreads];
@@ -318,7 +317,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const FwdArgs 
     const int begin = int((long long)sp.vecs * part / parts), end = int((long long)sp.vecs * (part + 1) / parts);
     // the single element in front of or behind the vectors that this thread owns, if any
     const int edge = (part == 0 && tid < sp.head) ? tid
-                     : (part == parts - 1 && tid >= 32 && tid < 32 + sp.tail) ? sp.head + sp.vecs * E + (tid - 32)
+                     : (part == parts - 1 && tid >= 16 && tid < 16 + sp.tail) ? sp.head + sp.vecs * E + (tid - 16)
                                                                               : -1;
     uint4 next[kUnroll];  // the next round's loads are under way while this one is added
     auto load_round = [&](int i0) {
@@ -809,8 +808,12 @@ cudaError_t launch_forward(const FwdArgs& a, cudaStream_t stream) {
         auto kern = a.V <= 128 ? token_logprobs_warp_kernel<T, 4> : a.V <= 384 ? token_logprobs_warp_kernel<T, 12> : token_logprobs_warp_kernel<T, 32>;
         return launch_pdl(kern, dim3((a.rows + rows - 1) / rows), dim3(kWarpRowThreads), 0, stream, a);
     }
-    // a thread should have some vectors of its row: short rows get small CTAs
-    return a.V <= kSmallRowVecs * Elem<T>::kPerVec ? launch_rows<T, 64>(a, stream) : launch_rows<T, 256>(a, stream);
+    // A thread should have some rounds of its row, and the ends of rows should not fall together on an SM: the shorter the row, the
+    // smaller (and the more) the CTAs. Measured with 64 / 128 / 256 threads, BF16, without and with 20 alternatives: 8192 x 6000
+    // 30 / 43 / - us, 4096 x 12000 25 and 42 / 21 and 36 / 29 and 51 us, 6001 x 50304 - / 98 and 121 / 104 and 137 us, 4096 x 131072 - / 195
+    // and 255 / 164 and 186 us.
+    const int vecs = a.V / Elem<T>::kPerVec;
+    return vecs <= kSmallRowVecs ? launch_rows<T, 64>(a, stream) : vecs <= kMiddleRowVecs ? launch_rows<T, 128>(a, stream) : launch_rows<T, 256>(a, stream);
 }
 
 template <typename T, int kThreads>
