@@ -77,6 +77,15 @@ def test_cache_shared_by_all_sequences(pkg):
     check(pkg.ops.attention_decode_bf16(q, k1, v1, ints([500, 77, 300]), 0.1), oracle(q, k1, v1, [500, 77, 300], 0.1))
 
 
+def test_empty_caches_and_no_sequences(pkg):
+    q, k, v = make(2, 0, 4, 2, 64)
+    out, lse = pkg.ops.attention_decode_bf16(q, k, v, ints([0, 5]), 0.1)
+    assert bool((out == 0).all()) and bool((lse == -math.inf).all())
+    q, k, v = make(0, 10, 4, 2, 64)
+    out, lse = pkg.ops.attention_decode_bf16(q, k, v, ints([]), 0.1)
+    assert out.shape == (0, 4, 64) and lse.shape == (0, 4)
+
+
 def test_lengths_are_clipped_and_results_repeat(pkg):
     q, k, v = make(2, 3000, 8, 2, 64, seed=3)
     a = pkg.ops.attention_decode_bf16(q, k, v, ints([3000, 0]), 0.125)
