@@ -113,7 +113,7 @@ def test_token_logprobs_refuse(pkg):
     for change in both + [dict(lp=None), dict(top=-1), dict(top=33), dict(top=20, V=19), dict(tl=None), dict(tt=None), dict(rows=1 << 30)]:
         assert logprobs(so, **change) == -1, change
         assert b"token_logprobs" in so.b200loss_last_error()
-    for change in both + [dict(g=None), dict(d=None), dict(ds=49), dict(d=ctypes.c_void_p(4097))]:
+    for change in both + [dict(g=None), dict(d=None), dict(ds=49), dict(rows=1 << 30), dict(d=ctypes.c_void_p(4097))]:
         assert logprobs_backward(so, **change) == -1, change
     assert logprobs(so, rows=0, x=None, t=None) == 0 and logprobs_backward(so, rows=0, x=None, d=None) == 0
 

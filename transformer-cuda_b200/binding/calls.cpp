@@ -12,7 +12,9 @@
 #include <ATen/ops/zeros.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/utils/object_ptr.h>
 
 #include <cstdarg>
 #include <cstdio>
@@ -118,11 +120,24 @@ at::Tensor zeros(c10::IntArrayRef sizes, at::ScalarType type, at::Device device)
 // Scratch of one call from torch's allocator: ordered with the stream, its own in every captured graph.
 at::Tensor scratch(int64_t bytes, at::Device device) { return empty({bytes > 16 ? bytes : 16}, at::kByte, device); }
 
-PyObject* own(PyObject* o) {
+// A new reference to `o`, and to a Python tensor around `t`.
+THPObjectPtr own(PyObject* o) {
     Py_INCREF(o);
+    return THPObjectPtr(o);
+}
+THPObjectPtr wrap(at::Tensor t) {
+    THPObjectPtr o(THPVariable_Wrap(std::move(t)));
+    if (!o) throw PyFailed{};
     return o;
 }
-PyObject* wrap(at::Tensor t) { return THPVariable_Wrap(std::move(t)); }
+template <typename... P>
+PyObject* tuple_of(P&&... items) {
+    THPObjectPtr t(PyTuple_New(sizeof...(items)));
+    if (!t) throw PyFailed{};
+    Py_ssize_t i = 0;
+    (PyTuple_SET_ITEM(t.get(), i++, items.release()), ...);
+    return t.release();
+}
 // The tuple of what `make` returns, or the Python error.
 template <typename F>
 PyObject* guarded(F&& f) {
@@ -130,8 +145,8 @@ PyObject* guarded(F&& f) {
         return f();
     } catch (const PyFailed&) {
         return nullptr;
-    } catch (const std::exception& e) {
-        if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what());
+    } catch (...) {  // torch's own errors (out of memory among them) in its own classes
+        torch::translate_exception_to_python(std::current_exception());
         return nullptr;
     }
 }
@@ -172,23 +187,17 @@ PyObject* ragged_forward(PyObject*, PyObject* const* p, Py_ssize_t np) {
         const float scale = to_float(p[4]);
         const at::Device device = a.q->device();
         const c10::cuda::CUDAGuard guard(device);
-        PyObject* out = p[5] == Py_None ? wrap(zeros(a.q->sizes(), at::kBFloat16, device)) : own(p[5]);
-        PyObject* lse = p[6] == Py_None ? wrap(zeros({a.H, a.total}, at::kFloat, device)) : own(p[6]);
-        try {
-            void* out_ptr;
-            const int64_t so = head_rows_like(out, "out", *a.q, &out_ptr);
-            float* lse_ptr = static_cast<float*>(vector(lse, Kind::kAttn, "lse", at::kFloat, (int64_t)a.H * a.total, device));
-            const long long bytes = b200attn_ragged_workspace_bytes(a.total, a.n, a.H, a.Hkv, a.d, 0);
-            const at::Tensor ws = scratch(bytes, device);
-            check_attn(b200attn_fwd_bf16_ragged(a.q->data_ptr(), a.k->data_ptr(), a.v->data_ptr(), static_cast<int*>(a.offsets), out_ptr, lse_ptr,
-                                                ws.data_ptr(), bytes, a.total, a.n, a.H, a.Hkv, a.d, a.sq, a.skv, so, scale,
-                                                c10::cuda::getCurrentCUDAStream(device.index()).stream()));
-        } catch (...) {
-            Py_DECREF(out);
-            Py_DECREF(lse);
-            throw;
-        }
-        return Py_BuildValue("(NN)", out, lse);
+        THPObjectPtr out = p[5] == Py_None ? wrap(zeros(a.q->sizes(), at::kBFloat16, device)) : own(p[5]);
+        THPObjectPtr lse = p[6] == Py_None ? wrap(zeros({a.H, a.total}, at::kFloat, device)) : own(p[6]);
+        void* out_ptr;
+        const int64_t so = head_rows_like(out, "out", *a.q, &out_ptr);
+        float* lse_ptr = static_cast<float*>(vector(lse, Kind::kAttn, "lse", at::kFloat, (int64_t)a.H * a.total, device));
+        const long long bytes = b200attn_ragged_workspace_bytes(a.total, a.n, a.H, a.Hkv, a.d, 0);
+        const at::Tensor ws = scratch(bytes, device);
+        check_attn(b200attn_fwd_bf16_ragged(a.q->data_ptr(), a.k->data_ptr(), a.v->data_ptr(), static_cast<int*>(a.offsets), out_ptr, lse_ptr,
+                                            ws.data_ptr(), bytes, a.total, a.n, a.H, a.Hkv, a.d, a.sq, a.skv, so, scale,
+                                            c10::cuda::getCurrentCUDAStream(device.index()).stream()));
+        return tuple_of(out, lse);
     });
 }
 
@@ -203,25 +212,18 @@ PyObject* ragged_backward(PyObject*, PyObject* const* p, Py_ssize_t np) {
         void *out_ptr, *dout_ptr, *dq_ptr, *dk_ptr, *dv_ptr;
         const int64_t so = head_rows_like(p[3], "out", *a.q, &out_ptr), sdo = head_rows_like(p[4], "dout", *a.q, &dout_ptr);
         float* lse_ptr = static_cast<float*>(vector(p[5], Kind::kAttn, "lse", at::kFloat, (int64_t)a.H * a.total, device));
-        PyObject* dq = p[8] == Py_None ? wrap(zeros(a.q->sizes(), at::kBFloat16, device)) : own(p[8]);
-        PyObject* dk = p[9] == Py_None ? wrap(zeros(a.k->sizes(), at::kBFloat16, device)) : own(p[9]);
-        PyObject* dv = p[10] == Py_None ? wrap(zeros(a.k->sizes(), at::kBFloat16, device)) : own(p[10]);
-        try {
-            const int64_t sdq = head_rows_like(dq, "dq", *a.q, &dq_ptr), sdk = head_rows_like(dk, "dk", *a.k, &dk_ptr);
-            if (head_rows_like(dv, "dv", *a.k, &dv_ptr) != sdk) refuse(Kind::kAttn, "dk and dv must have the same row stride");
-            const long long bytes = b200attn_ragged_workspace_bytes(a.total, a.n, a.H, a.Hkv, a.d, 1);
-            const at::Tensor ws = scratch(bytes, device);
-            check_attn(b200attn_bwd_bf16_ragged(a.q->data_ptr(), a.k->data_ptr(), a.v->data_ptr(), out_ptr, dout_ptr, lse_ptr,
-                                                static_cast<int*>(a.offsets), dq_ptr, dk_ptr, dv_ptr, ws.data_ptr(), bytes, a.total, a.n, a.H,
-                                                a.Hkv, a.d, a.sq, a.skv, so, sdo, sdq, sdk, scale,
-                                                c10::cuda::getCurrentCUDAStream(device.index()).stream()));
-        } catch (...) {
-            Py_DECREF(dq);
-            Py_DECREF(dk);
-            Py_DECREF(dv);
-            throw;
-        }
-        return Py_BuildValue("(NNN)", dq, dk, dv);
+        THPObjectPtr dq = p[8] == Py_None ? wrap(zeros(a.q->sizes(), at::kBFloat16, device)) : own(p[8]);
+        THPObjectPtr dk = p[9] == Py_None ? wrap(zeros(a.k->sizes(), at::kBFloat16, device)) : own(p[9]);
+        THPObjectPtr dv = p[10] == Py_None ? wrap(zeros(a.k->sizes(), at::kBFloat16, device)) : own(p[10]);
+        const int64_t sdq = head_rows_like(dq, "dq", *a.q, &dq_ptr), sdk = head_rows_like(dk, "dk", *a.k, &dk_ptr);
+        if (head_rows_like(dv, "dv", *a.k, &dv_ptr) != sdk) refuse(Kind::kAttn, "dk and dv must have the same row stride");
+        const long long bytes = b200attn_ragged_workspace_bytes(a.total, a.n, a.H, a.Hkv, a.d, 1);
+        const at::Tensor ws = scratch(bytes, device);
+        check_attn(b200attn_bwd_bf16_ragged(a.q->data_ptr(), a.k->data_ptr(), a.v->data_ptr(), out_ptr, dout_ptr, lse_ptr,
+                                            static_cast<int*>(a.offsets), dq_ptr, dk_ptr, dv_ptr, ws.data_ptr(), bytes, a.total, a.n, a.H,
+                                            a.Hkv, a.d, a.sq, a.skv, so, sdo, sdq, sdk, scale,
+                                            c10::cuda::getCurrentCUDAStream(device.index()).stream()));
+        return tuple_of(dq, dk, dv);
     });
 }
 
@@ -251,24 +253,18 @@ PyObject* decode(PyObject*, PyObject* const* p, Py_ssize_t np) {
         const float scale = to_float(p[4]);
         int* lengths = static_cast<int*>(vector(p[3], Kind::kAttn, "lengths", at::kInt, B, device));
         const c10::cuda::CUDAGuard guard(device);
-        PyObject* out = p[5] == Py_None ? wrap(empty({B, H, d}, at::kBFloat16, device)) : own(p[5]);
-        PyObject* lse = p[6] == Py_None ? wrap(empty({B, H}, at::kFloat, device)) : own(p[6]);
-        try {
-            void* out_ptr = vector(out, Kind::kAttn, "out", at::kBFloat16, (int64_t)B * H * d, device);
-            float* lse_ptr = static_cast<float*>(vector(lse, Kind::kAttn, "lse", at::kFloat, (int64_t)B * H, device));
-            const long long bytes = b200attn_decode_workspace_bytes(B, T, H, Hkv, d);
-            at::Tensor ws;
-            if (bytes) ws = scratch(bytes, device);
-            check_attn(b200attn_decode_bf16(q.data_ptr(), cache[0]->data_ptr(), cache[1]->data_ptr(), lengths, out_ptr, lse_ptr,
-                                            bytes ? ws.data_ptr() : nullptr, bytes, B, T, H, Hkv, d, sq, strides[0][0], strides[0][1], strides[0][2],
-                                            strides[1][0], strides[1][1], strides[1][2], scale,
-                                            c10::cuda::getCurrentCUDAStream(device.index()).stream()));
-        } catch (...) {
-            Py_DECREF(out);
-            Py_DECREF(lse);
-            throw;
-        }
-        return Py_BuildValue("(NN)", out, lse);
+        THPObjectPtr out = p[5] == Py_None ? wrap(empty({B, H, d}, at::kBFloat16, device)) : own(p[5]);
+        THPObjectPtr lse = p[6] == Py_None ? wrap(empty({B, H}, at::kFloat, device)) : own(p[6]);
+        void* out_ptr = vector(out, Kind::kAttn, "out", at::kBFloat16, (int64_t)B * H * d, device);
+        float* lse_ptr = static_cast<float*>(vector(lse, Kind::kAttn, "lse", at::kFloat, (int64_t)B * H, device));
+        const long long bytes = b200attn_decode_workspace_bytes(B, T, H, Hkv, d);
+        at::Tensor ws;
+        if (bytes) ws = scratch(bytes, device);
+        check_attn(b200attn_decode_bf16(q.data_ptr(), cache[0]->data_ptr(), cache[1]->data_ptr(), lengths, out_ptr, lse_ptr,
+                                        bytes ? ws.data_ptr() : nullptr, bytes, B, T, H, Hkv, d, sq, strides[0][0], strides[0][1], strides[0][2],
+                                        strides[1][0], strides[1][1], strides[1][2], scale,
+                                        c10::cuda::getCurrentCUDAStream(device.index()).stream()));
+        return tuple_of(out, lse);
     });
 }
 
@@ -322,8 +318,8 @@ PyObject* token_logprobs(PyObject*, PyObject* const* p, Py_ssize_t np) {
                                            static_cast<float*>(entropy.data_ptr()), static_cast<float*>(stats.data_ptr()), int(top),
                                            top ? static_cast<float*>(top_logprobs.data_ptr()) : nullptr, top ? static_cast<int*>(top_tokens.data_ptr()) : nullptr,
                                            c10::cuda::getCurrentCUDAStream(device.index()).stream()));
-        return Py_BuildValue("(NNNNN)", wrap(std::move(logprobs)), wrap(std::move(entropy)), wrap(std::move(stats)),
-                             top ? wrap(std::move(top_logprobs)) : own(Py_None), top ? wrap(std::move(top_tokens)) : own(Py_None));
+        return tuple_of(wrap(std::move(logprobs)), wrap(std::move(entropy)), wrap(std::move(stats)),
+                        top ? wrap(std::move(top_logprobs)) : own(Py_None), top ? wrap(std::move(top_tokens)) : own(Py_None));
     });
 }
 
@@ -341,7 +337,7 @@ PyObject* token_logprobs_backward(PyObject*, PyObject* const* p, Py_ssize_t np) 
         const float* ge = p[5] == Py_None ? nullptr : static_cast<float*>(vector(p[5], Kind::kLoss, "grad_entropy", at::kFloat, r.rows, device));
         const float temperature = to_float(p[6]);
         const c10::cuda::CUDAGuard guard(device);
-        PyObject* result;
+        THPObjectPtr result;
         int64_t d_stride = r.V;
         if (p[7] == Py_None) {
             result = wrap(empty(x.sizes(), x.scalar_type(), device));
@@ -352,15 +348,10 @@ PyObject* token_logprobs_backward(PyObject*, PyObject* const* p, Py_ssize_t np) 
             if (d.data_ptr() == x.data_ptr() && d_stride != r.stride) refuse(Kind::kLoss, "dlogits in the logits' place must have the logits' row stride");
             result = own(p[7]);
         }
-        try {
-            check_loss(b200loss_token_logprobs_backward(x.data_ptr(), r.dtype, r.stride, targets, entropy, stats, g, ge, r.rows, r.V, temperature,
-                                                        THPVariable_Unpack(result).data_ptr(), d_stride,
-                                                        c10::cuda::getCurrentCUDAStream(device.index()).stream()));
-        } catch (...) {
-            Py_DECREF(result);
-            throw;
-        }
-        return result;
+        check_loss(b200loss_token_logprobs_backward(x.data_ptr(), r.dtype, r.stride, targets, entropy, stats, g, ge, r.rows, r.V, temperature,
+                                                    THPVariable_Unpack(result.get()).data_ptr(), d_stride,
+                                                    c10::cuda::getCurrentCUDAStream(device.index()).stream()));
+        return result.release();
     });
 }
 
@@ -371,9 +362,9 @@ PyObject* set_errors(PyObject*, PyObject* const* p, Py_ssize_t np) {
         for (int i = 0; i < 2; ++i) {
             PyObject*& slot = i ? g_loss_error : g_attn_error;
             Py_XDECREF(slot);
-            slot = own(p[i]);
+            slot = own(p[i]).release();
         }
-        return own(Py_None);
+        return own(Py_None).release();
     });
 }
 

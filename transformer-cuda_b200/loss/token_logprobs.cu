@@ -819,7 +819,7 @@ cudaError_t launch_forward(const FwdArgs& a, cudaStream_t stream) {
 template <typename T, int kThreads>
 cudaError_t launch_gradient(BwdArgs a, cudaStream_t stream) {
     constexpr int per_cta = kThreads * kUnroll * Elem<T>::kPerVec;
-    a.chunks = (a.V + per_cta - 1) / per_cta;
+    a.chunks = int((a.V + (long long)per_cta - 1) / per_cta);
     if ((long long)a.rows * a.chunks > 0x7fffffffLL) return cudaErrorInvalidValue;
     // launched the ordinary way: its many short CTAs pay more for the dependency wait than the overlap gives (8192 x 3000: 21 us, 17 so)
     token_logprobs_bwd_kernel<T, kThreads><<<unsigned(a.rows) * unsigned(a.chunks), kThreads, 0, stream>>>(a);
@@ -865,6 +865,7 @@ int b200loss_token_logprobs_backward(const void* logits, int dtype, long long ro
     if (d_row_stride < V) return fail(B200LOSS_ERR_ARG, "b200loss_token_logprobs_backward: d_row_stride is smaller than V");
     if (rows == 0) return B200LOSS_OK;
     const size_t size = dtype == B200LOSS_F32 ? 4 : 2;
+    if (rows > 0x7fffffff / kMaxCluster) return fail(B200LOSS_ERR_ARG, "b200loss_token_logprobs_backward: too many rows");
     if (misaligned(logits, size) || misaligned(dlogits, size))
         return fail(B200LOSS_ERR_ARG, "b200loss_token_logprobs_backward: logits or dlogits are not aligned to their type");
     BwdArgs a{logits, row_stride, targets, entropy, stats, grad_logprobs, grad_entropy, rows, V, 1.0f / temperature, dlogits, d_row_stride, 1};
