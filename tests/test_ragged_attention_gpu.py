@@ -106,8 +106,18 @@ def test_a_spoilt_sequence_spoils_no_other(pkg, d, bad):
 
 
 @pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lengths,H,Hkv", [([100 + 7 * i for i in range(20)], 6, 2), ([40, 900], 32, 8), ([700, 650, 500], 18, 2)], ids=["twenty", "two", "three"])
+def test_other_grid_sizes(pkg, lengths, H, Hkv, d):
+    """Grids between one and two CTAs per SM of short and of long sequences, and larger ones."""
+    q, k, v, dout, offsets = make(lengths, H, Hkv, d, seed=14)
+    got = run(pkg.ops, q, k, v, dout, offsets, 0.1)
+    assert_close(got, *attention(q, k, v, lengths, 0.1, dout), NAMES)
+
+
+@pytest.mark.parametrize("d", [64, 128])
 def test_equal_lengths_agree_with_the_dense_path(pkg, d):
-    B, H, T = 3, 2, 256
+    """Bit by bit where both take the forward variant with two CTAs per SM: from 297 tiles and heads on."""
+    B, H, T = 80, 2, 256
     q, k, v, dout, offsets = make([T] * B, H, H, d, seed=7, fused=False)
     got = run(pkg.ops, q, k, v, dout, offsets, 0.125)
     slab = lambda t: t.view(B, T, H, d).transpose(1, 2).contiguous()

@@ -26,6 +26,7 @@
 // Every mbarrier wait has an iteration limit (tc_common.cuh); a wait that gives up sets the fault
 // word and the kernel still runs to its end and frees its TMEM.
 #include "kernels.cuh"
+#include "ragged_items.cuh"
 #include "tc_common.cuh"
 
 
@@ -62,7 +63,8 @@ struct FwdBarriers {
     uint64_t o_done;
 };
 
-template <int D, bool OUT_F32>
+// RAGGED: packed sequences with grouped heads, where the card is not full; every CTA finds its tile in the offsets.
+template <int D, bool OUT_F32, bool RAGGED>
 __global__ void __launch_bounds__(kThreads, 1) attn_fwd_tc_kernel(const __grid_constant__ TcFwdArgs a) {
     using Cfg = FwdCfg<D>;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -83,10 +85,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd_tc_kernel(const __grid_c
     const int n_q_tiles = (a.T + kBM - 1) / kBM;
     // CTA order: the last query tile of a slab is the longest. Longest-first across all slabs when the
     // problem fits in L2 (shortest tail), else slab by slab (resident CTAs share K/V tiles in L2).
-    const int bh = a.tile_major_order ? int(blockIdx.x % a.BH) : int(blockIdx.x / n_q_tiles);
-    const int qt = n_q_tiles - 1 - (a.tile_major_order ? int(blockIdx.x / a.BH) : int(blockIdx.x % n_q_tiles));
-    const int hh = bh % a.H, bb = bh / a.H;  // head and batch coordinates of the 4-D tensor maps
-    const int n_kv = qt + 1;                                  // key tiles 0..qt; qt is the diagonal tile
+    int bh = 0, qt = 0, hh = 0, bb = 0, hk = 0;  // hh, bb: head and batch coordinates of the 4-D tensor maps; hk: key head
+    int row0 = 0, valid = kBM;                   // RAGGED: first row of the sequence, rows of this tile that belong to it
+    if constexpr (!RAGGED) {
+        bh = a.tile_major_order ? int(blockIdx.x % a.BH) : int(blockIdx.x / n_q_tiles);
+        qt = n_q_tiles - 1 - (a.tile_major_order ? int(blockIdx.x / a.BH) : int(blockIdx.x % n_q_tiles));
+        hh = bh % a.H, bb = bh / a.H, hk = hh;
+    }
 
     if (tid == 0) {
         mbar_init(&bars.q_full, 1);
@@ -106,6 +111,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd_tc_kernel(const __grid_c
         mbar_fence_init();
     }
     if (warp == kProducerWarp) {
+        if (RAGGED && lane == 0) {  // under the set-up
+            tma_prefetch_desc(&a.map_q);
+            tma_prefetch_desc(&a.map_k);
+            tma_prefetch_desc(&a.map_v);
+        }
         tmem_alloc(&tmem_base_slot, Cfg::kTmemCols);
         tmem_relinquish();
     }
@@ -116,27 +126,40 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd_tc_kernel(const __grid_c
     // barriers, TMEM and the tensor maps are set up: from here on global memory is touched, so wait for the
     // kernel in front of this one in the stream (returns at once for an ordinary launch)
     pdl_wait();
+    if constexpr (RAGGED) {
+        const int4 w = ragged_find(a.ragged.offsets, a.ragged.n, a.T, int(blockIdx.x / unsigned(a.H)), lane);
+        if (w.z == 0) {  // the host knows an upper bound only
+            __syncthreads();
+            if (warp == kProducerWarp) tmem_dealloc(tmem, Cfg::kTmemCols);
+            return;
+        }
+        bh = hh = int(blockIdx.x % unsigned(a.H)), hk = hh / a.ragged.group;
+        row0 = w.x, qt = w.z - 1, valid = min(kBM, w.y - qt * kBM);
+    }
+    const int n_kv = qt + 1;  // key tiles 0..qt; qt is the diagonal tile
 
     if (warp == kProducerWarp) {
         // ------------------------------------------------------------ TMA producer
         if (lane == 0) {
-            tma_prefetch_desc(&a.map_q);
-            tma_prefetch_desc(&a.map_k);
-            tma_prefetch_desc(&a.map_v);
+            if (!RAGGED) {
+                tma_prefetch_desc(&a.map_q);
+                tma_prefetch_desc(&a.map_k);
+                tma_prefetch_desc(&a.map_v);
+            }
             mbar_expect_tx(&bars.q_full, Cfg::kTileBytes);
             for (int at = 0; at < Cfg::kAtoms; ++at)
-                tma_load_4d(sQ + at * kAtomBytes, &a.map_q, &bars.q_full, at * 64, qt * kBM, hh, bb);
+                tma_load_4d(sQ + at * kAtomBytes, &a.map_q, &bars.q_full, at * 64, row0 + qt * kBM, hh, bb);
             for (int j = 0; j < n_kv; ++j) {
                 const int ks = j % Cfg::kKStages, kround = j / Cfg::kKStages;
                 if (kround > 0) mbar_wait(&bars.k_empty[ks], (kround - 1) & 1, &abort_flag, a.fault_word, 0x10);
                 mbar_expect_tx(&bars.k_full[ks], Cfg::kTileBytes);
                 for (int at = 0; at < Cfg::kAtoms; ++at)
-                    tma_load_4d(sK + ks * Cfg::kTileBytes + at * kAtomBytes, &a.map_k, &bars.k_full[ks], at * 64, j * kBN, hh, bb);
+                    tma_load_4d(sK + ks * Cfg::kTileBytes + at * kAtomBytes, &a.map_k, &bars.k_full[ks], at * 64, row0 + j * kBN, hk, bb);
                 const int vs = j % Cfg::kVStages, vround = j / Cfg::kVStages;
                 if (vround > 0) mbar_wait(&bars.v_empty[vs], (vround - 1) & 1, &abort_flag, a.fault_word, 0x11);
                 mbar_expect_tx(&bars.v_full[vs], Cfg::kTileBytes);
                 for (int at = 0; at < Cfg::kAtoms; ++at)
-                    tma_load_4d(sV + vs * Cfg::kTileBytes + at * kAtomBytes, &a.map_v, &bars.v_full[vs], at * 64, j * kBN, hh, bb);
+                    tma_load_4d(sV + vs * Cfg::kTileBytes + at * kAtomBytes, &a.map_v, &bars.v_full[vs], at * 64, row0 + j * kBN, hk, bb);
             }
         }
         __syncwarp();
@@ -172,6 +195,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd_tc_kernel(const __grid_c
             const int vs = j % Cfg::kVStages;
             const int b = j % Cfg::kSBuffers;
             mbar_wait(&bars.v_full[vs], (j / Cfg::kVStages) & 1, &abort_flag, a.fault_word, 0x22);
+            if constexpr (RAGGED) {  // keys behind the sequence have P = 0, whatever their values hold
+                if (j == qt && valid < kBN) zero_tile_rows<128>(sV + vs * Cfg::kTileBytes, Cfg::kAtoms, valid, lane);
+            }
             mbar_wait(&bars.p_full[b], (j / Cfg::kSBuffers) & 1, &abort_flag, a.fault_word, 0x23);
             tc_fence_after();
             if (elect_one()) {
@@ -278,9 +304,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd_tc_kernel(const __grid_c
         mbar_wait(&bars.o_done, (n_kv - 1) & 1, &abort_flag, a.fault_word, 0x32);
         tc_fence_after();
         const float inv_l = 1.0f / l_run;
-        const int row_g = qt * kBM + r;
+        const int row_g = row0 + qt * kBM + r;
+        const bool in_range = RAGGED ? r < valid : row_g < a.T;
         const long long stat_idx = (long long)bh * a.T + row_g;
-        if (row_g < a.T && half == 0) {
+        if (in_range && half == 0) {
             // exported statistics are relative to the true row maximum
             if (a.m_out) a.m_out[stat_idx] = m_true * kLn2;
             if (a.l_out) a.l_out[stat_idx] = l_run * exp2f(m_ref - m_true);
@@ -292,7 +319,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd_tc_kernel(const __grid_c
             tmem_ld32(tmem_addr(tmem, lane_base, Cfg::kColO + c), ov);
             tmem_wait_ld();
             if constexpr (OUT_F32) {
-                if (row_g < a.T) {
+                if (in_range) {
                     float* dst = reinterpret_cast<float*>(a.out) + ((long long)bh * a.T + row_g) * D + c;
 #pragma unroll
                     for (int i = 0; i < 32; i += 4)
@@ -310,15 +337,21 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd_tc_kernel(const __grid_c
                     w.y = pack_bf16x2(__uint_as_float(ov[i + 2]) * inv_l, __uint_as_float(ov[i + 3]) * inv_l);
                     w.z = pack_bf16x2(__uint_as_float(ov[i + 4]) * inv_l, __uint_as_float(ov[i + 5]) * inv_l);
                     w.w = pack_bf16x2(__uint_as_float(ov[i + 6]) * inv_l, __uint_as_float(ov[i + 7]) * inv_l);
-                    *reinterpret_cast<uint4*>(atom + swz128(r, ((c & 63) + i) >> 3)) = w;
+                    if (RAGGED && valid < kBM) {  // the rows behind the sequence are not this tile's to write
+                        if (in_range)
+                            *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(a.out) + (long long)row_g * a.ragged.out_stride +
+                                                      (long long)hh * D + c + i) = w;
+                    } else {
+                        *reinterpret_cast<uint4*>(atom + swz128(r, ((c & 63) + i) >> 3)) = w;
+                    }
                 }
             }
         }
-        if constexpr (!OUT_F32) {
+        if (!OUT_F32 && !(RAGGED && valid < kBM)) {
             fence_proxy_async_smem();
             named_bar_sync(1, kSoftmaxThreads);
             if (tid == 0) {
-                for (int at = 0; at < Cfg::kAtoms; ++at) tma_store_4d(&a.map_o, sQ + at * kAtomBytes, at * 64, qt * kBM, hh, bb);
+                for (int at = 0; at < Cfg::kAtoms; ++at) tma_store_4d(&a.map_o, sQ + at * kAtomBytes, at * 64, row0 + qt * kBM, hh, bb);
                 tma_store_commit();
                 tma_store_wait_read();  // the staging tile must outlive the bulk read; the write completes with the grid
             }
@@ -332,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_fwd_tc_kernel(const __grid_c
 template <int D, bool OUT_F32>
 cudaError_t launch_fwd(const TcFwdArgs& a, cudaStream_t stream) {
     using Cfg = FwdCfg<D>;
-    auto kern = attn_fwd_tc_kernel<D, OUT_F32>;
+    auto kern = attn_fwd_tc_kernel<D, OUT_F32, false>;
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
     if (e != cudaSuccess) return e;
     const int n_q_tiles = (a.T + kBM - 1) / kBM;
@@ -340,7 +373,29 @@ cudaError_t launch_fwd(const TcFwdArgs& a, cudaStream_t stream) {
     return launch_pdl(kern, dim3((unsigned int)blocks), dim3(kThreads), Cfg::kSmemBytes, stream, a);
 }
 
+template <int D>
+cudaError_t launch_fwd_ragged(const TcFwdArgs& a, cudaStream_t stream) {
+    using Cfg = FwdCfg<D>;
+    auto kern = attn_fwd_tc_kernel<D, false, true>;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmemBytes);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(kern, dim3((unsigned int)(a.ragged.capacity * a.H)), dim3(kThreads), Cfg::kSmemBytes, stream, a);
+}
+
 }  // namespace
+
+cudaError_t launch_attn_fwd_ragged(const TcFwdArgs& a, cudaStream_t stream) {
+    // Where the card is not full the chain of a tile's steps is what counts, and this variant (eight softmax warps, scores made two
+    // tiles ahead) has the shorter one; sequences of one or two tiles gain from two CTAs per SM again as soon as the tiles outnumber
+    // the SMs clearly. Measured, two small CTAs / one large, d = 128: one sequence of 4000, 2 heads 58 / 37 us; two of 1538, 8 heads
+    // (208 CTAs) 30 / 21 us; one of 1700, 20 heads (280) 34 / 27 us; twenty of 60-300, 6 heads (270) 12.3 / 14.5 us.
+    const long long ctas = (long long)a.ragged.capacity * a.H;
+    if (a.ragged.items == nullptr && (ctas <= 222 || a.T >= 256ll * a.ragged.n)) {
+        if (a.d == 64) return launch_fwd_ragged<64>(a, stream);
+        if (a.d == 128) return launch_fwd_ragged<128>(a, stream);
+    }
+    return launch_attn_fwd_ragged_short(a, stream);
+}
 
 cudaError_t launch_attn_fwd_tc(const TcFwdArgs& a, cudaStream_t stream) {
     if (a.BH == 0 || a.T == 0) return cudaSuccess;

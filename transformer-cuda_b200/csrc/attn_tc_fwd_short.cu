@@ -397,7 +397,7 @@ cudaError_t launch_fwd_ragged(const TcFwdArgs& a, cudaStream_t stream) {
 
 }  // namespace
 
-cudaError_t launch_attn_fwd_ragged(const TcFwdArgs& a, cudaStream_t stream) {
+cudaError_t launch_attn_fwd_ragged_short(const TcFwdArgs& a, cudaStream_t stream) {
     if (a.d == 64) return launch_fwd_ragged<64>(a, stream);
     if (a.d == 128) return launch_fwd_ragged<128>(a, stream);
     return cudaErrorInvalidValue;

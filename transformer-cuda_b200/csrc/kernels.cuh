@@ -142,7 +142,8 @@ struct TcFwdArgs {
 };
 cudaError_t launch_attn_fwd_tc(const TcFwdArgs& a, cudaStream_t stream);        // picks the variant by T
 cudaError_t launch_attn_fwd_tc_short(const TcFwdArgs& a, cudaStream_t stream);  // two CTAs per SM (d = 64; d = 128 up to T = 4096)
-cudaError_t launch_attn_fwd_ragged(const TcFwdArgs& a, cudaStream_t stream);    // packed sequences, BF16 output
+cudaError_t launch_attn_fwd_ragged(const TcFwdArgs& a, cudaStream_t stream);    // packed sequences, BF16 output: picks the variant
+cudaError_t launch_attn_fwd_ragged_short(const TcFwdArgs& a, cudaStream_t stream);
 
 struct TcBwdArgs {
     CUtensorMap map_q, map_k, map_v, map_do;  // BF16
