@@ -305,13 +305,13 @@ __global__ void __launch_bounds__(kThreads, 2) attn_decode_kernel(const DecodeAr
 }
 
 // One CTA per (sequence, head): joins the splits that hold keys. The sums are added in an order that depends on their number only.
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 512;  // a warp reads a split's sums at once; each has few splits, all under way together
 constexpr int kMaxSplits = 256;
 template <int D>
 __global__ void __launch_bounds__(kJoinThreads) attn_decode_join_kernel(const DecodeArgs a) {
-    constexpr int kGroups = kJoinThreads / (D / 2);
+    constexpr int kGroups = kJoinThreads / 32, kVec = D / 32;
     __shared__ float s_f[kMaxSplits];
-    __shared__ float2 s_x[kGroups][D / 2];
+    __shared__ float s_x[kGroups][D];
     __shared__ float s_red[2][kJoinThreads / 32];
     pdl_launch_dependents();
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_decode_join_kernel(const De
 #pragma unroll
     for (int w = 0; w < kJoinThreads / 32; ++w) M = fmaxf(M, s_red[0][w]);
     const float f = fast_exp2(ml.x - M);
-    s_f[tid] = f;
+    if (tid < kMaxSplits) s_f[tid] = f;
     float L = ml.y * f;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
@@ -337,19 +337,26 @@ __global__ void __launch_bounds__(kJoinThreads) attn_decode_join_kernel(const De
     L = 0.f;
 #pragma unroll
     for (int w = 0; w < kJoinThreads / 32; ++w) L += s_red[1][w];
-    const int grp = tid / (D / 2), e = tid % (D / 2);
-    float x0 = 0.f, x1 = 0.f;
-#pragma unroll 4
-    for (int i = grp; i < n; i += kGroups) {
-        const float2 x = *reinterpret_cast<const float2*>(a.part_o + (part + i) * D + 2 * e);
-        x0 = fmaf(x.x, s_f[i], x0), x1 = fmaf(x.y, s_f[i], x1);
-    }
-    s_x[grp][e] = make_float2(x0, x1);
-    __syncthreads();
-    if (grp == 0) {
+    float x[kVec];
 #pragma unroll
-        for (int i = 1; i < kGroups; ++i) x0 += s_x[i][e].x, x1 += s_x[i][e].y;
-        write_out(a, b, h, D, 2 * e, M, L, x0, x1);
+    for (int c = 0; c < kVec; ++c) x[c] = 0.f;
+#pragma unroll 8
+    for (int i = warp; i < n; i += kGroups) {
+        const float* from = a.part_o + (part + i) * D + lane * kVec;
+        float y[kVec];
+        if constexpr (kVec == 4) *reinterpret_cast<float4*>(y) = *reinterpret_cast<const float4*>(from);
+        else *reinterpret_cast<float2*>(y) = *reinterpret_cast<const float2*>(from);
+#pragma unroll
+        for (int c = 0; c < kVec; ++c) x[c] = fmaf(y[c], s_f[i], x[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < kVec; ++c) s_x[warp][lane * kVec + c] = x[c];
+    __syncthreads();
+    if (tid < D / 2) {
+        float x0 = 0.f, x1 = 0.f;
+#pragma unroll
+        for (int i = 0; i < kGroups; ++i) x0 += s_x[i][2 * tid], x1 += s_x[i][2 * tid + 1];
+        write_out(a, b, h, D, 2 * tid, M, L, x0, x1);
     }
 }
 
