@@ -116,6 +116,18 @@ def test_tokens_that_are_not_allowed(lo, V, dtype):
     assert r.entropy[0] == 0 and r.entropy[1] == 0 and r.logprobs[0] == -INF and r.logprobs[1] == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [33, 3001])
+@pytest.mark.parametrize("tau,weight", [(1e-6, 1.0), (1e-3, 1.0), (1.0, 1e12), (1e6, 1.0)])
+def test_masked_tokens_at_the_ends_of_the_temperature(lo, V, dtype, tau, weight):
+    """A masked logit's gradient is 0 however large the factors beside its probability are."""
+    x, t, g, ge = make(10, V, dtype, seed=V, std=3.0 * tau)
+    x[1::3, 1::2] = -INF
+    x[2::3, ::2] = torch.finfo(dtype).min
+    t[1::3], t[2::3] = 2, 1
+    check(lo, x, t, tau, 3, g, ge * weight)
+
+
 @pytest.mark.parametrize("V", [50, 4000])
 @pytest.mark.parametrize("bad", [float("nan"), INF])
 def test_spoilt_rows(lo, V, bad):

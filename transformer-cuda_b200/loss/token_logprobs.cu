@@ -662,6 +662,7 @@ struct BwdArgs {
     void* dlogits;
     long long d_row_stride;
     int chunks;  // CTAs per row
+    float lowest;  // d = x - m is held above this: 2^(c d - l) is 0 there already, and b d a number at every temperature and weight
 };
 
 // dx_v = p_v (a + b d) + [v = target] g / temperature with d = x_v - m and p_v = 2^(c d - l): one exponential and two
@@ -685,8 +686,8 @@ __device__ __forceinline__ RowGrad row_grad(const BwdArgs& p, int r) {
     q.b = -p.inv_temperature * p.inv_temperature * ge;
     return q;
 }
-__device__ __forceinline__ float grad_of(const RowGrad& q, float x, float c) {  // without the target's own term
-    const float d = max_nan(x - q.m, kLowest);
+__device__ __forceinline__ float grad_of(const RowGrad& q, float x, float c, float lowest) {  // without the target's own term
+    const float d = max_nan(x - q.m, lowest);
     return ex2(fmaf(d, c, -q.l)) * fmaf(d, q.b, q.a);
 }
 
@@ -724,7 +725,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_bwd_kernel(const BwdA
                 float x[E];
                 Elem<T>::unpack(w[u], x);
 #pragma unroll
-                for (int e = 0; e < E; ++e) x[e] = grad_of(q, x[e], c);
+                for (int e = 0; e < E; ++e) x[e] = grad_of(q, x[e], c, a.lowest);
                 const int at = q.target - (sp.head + i * E);
                 if ((unsigned)at < (unsigned)E) {
 #pragma unroll
@@ -739,7 +740,7 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_bwd_kernel(const BwdA
     const int edge = (chunk == 0 && tid < sp.head) ? tid
                      : (chunk == a.chunks - 1 && tid >= 32 && tid < 32 + sp.tail) ? sp.head + sp.vecs * E + (tid - 32)
                                                                                   : -1;
-    if (edge >= 0) Elem<T>::store(out + edge, q.zero ? 0.f : grad_of(q, Elem<T>::load(row + edge), c) + (edge == q.target ? q.g : 0.f));
+    if (edge >= 0) Elem<T>::store(out + edge, q.zero ? 0.f : grad_of(q, Elem<T>::load(row + edge), c, a.lowest) + (edge == q.target ? q.g : 0.f));
 }
 
 // One warp per row: short rows, and rows of dlogits at another distance from a 16-byte boundary than the logits'.
@@ -766,7 +767,7 @@ __global__ void __launch_bounds__(kWarpRowThreads) token_logprobs_bwd_warp_kerne
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
             const int v = v0 + u * 32 + lane;
-            if (v < a.V) Elem<T>::store(out + v, q.zero ? 0.f : grad_of(q, x[u], c) + (v == q.target ? q.g : 0.f));
+            if (v < a.V) Elem<T>::store(out + v, q.zero ? 0.f : grad_of(q, x[u], c, a.lowest) + (v == q.target ? q.g : 0.f));
         }
     }
 }
@@ -868,7 +869,7 @@ int b200loss_token_logprobs_backward(const void* logits, int dtype, long long ro
     if (rows > 0x7fffffff / kMaxCluster) return fail(B200LOSS_ERR_ARG, "b200loss_token_logprobs_backward: too many rows");
     if (misaligned(logits, size) || misaligned(dlogits, size))
         return fail(B200LOSS_ERR_ARG, "b200loss_token_logprobs_backward: logits or dlogits are not aligned to their type");
-    BwdArgs a{logits, row_stride, targets, entropy, stats, grad_logprobs, grad_entropy, rows, V, 1.0f / temperature, dlogits, d_row_stride, 1};
+    BwdArgs a{logits, row_stride, targets, entropy, stats, grad_logprobs, grad_entropy, rows, V, 1.0f / temperature, dlogits, d_row_stride, 1, -200.f * temperature * kLn2};
     return finish(dtype == B200LOSS_F32 ? launch_backward<float>(a, (cudaStream_t)stream) : launch_backward<__nv_bfloat16>(a, (cudaStream_t)stream),
                   "b200loss_token_logprobs_backward");
 }
