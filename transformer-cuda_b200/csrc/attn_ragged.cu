@@ -1,6 +1,6 @@
 // The passes around the attention kernels for packed sequences of different lengths: the list of work items, the backward's
 // pre-pass over O and dO, and the conversion of the dQ sums. (The attention itself: the RAGGED instances of
-// attn_tc_fwd_short.cu, attn_tc_bwd.cu and attn_tc_bwd64.cu.)
+// attn_tc_fwd_short.cu, attn_tc_fwd.cu, attn_tc_bwd.cu and attn_tc_bwd64.cu.)
 #include "kernels.cuh"
 #include "ragged_items.cuh"
 #include "tc_common.cuh"
@@ -80,13 +80,14 @@ __device__ void make_plan(const RaggedWork& w, int T, int shift, PlanShared& sh)
         at_item += count;
     }
     __syncthreads();
-    // offsets that are not in ascending order could make more items than fit: those behind the list are dropped
+    // offsets that are not in ascending order could make more items than fit: those behind the list are dropped (unsigned,
+    // so that a count that passes 2^31 stays behind the list; one that passes 2^32 has filled the list before it wraps)
     for_items([&](int row, int len, int c) {
         const int at = atomicAdd(&sh.level[levels - 1 - ((c - 1) >> shift)], 1);
-        if (at < w.capacity) w.items[at] = make_int4(row, len, c, 0);
+        if (unsigned(at) < unsigned(w.capacity)) w.items[at] = make_int4(row, len, c, 0);
     });
     if (tid == 0) {
-        w.count[0] = min(sh.total, w.capacity);
+        w.count[0] = int(min(unsigned(sh.total), unsigned(w.capacity)));
         w.count[1] = 0;
     }
 }
