@@ -79,7 +79,7 @@ def check(lo, x, t, tau=1.0, top=0, g=None, ge=None, **kw):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("V", [1, 2, 65, 1000, 1024, 1025, 2049, 5003, 50257, 131072])
+@pytest.mark.parametrize("V", [1, 2, 65, 300, 1000, 1024, 1025, 2049, 5003, 14001, 20011, 50257, 131072])
 @pytest.mark.parametrize("rows,tau", [(1, 1.0), (9, 0.7), (300, 1.5)])
 def test_forward_and_backward(lo, V, rows, dtype, tau):
     x, t, g, ge = make(rows, V, dtype, seed=V + rows)
@@ -88,9 +88,17 @@ def test_forward_and_backward(lo, V, rows, dtype, tau):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("V", [7, 1500, 40000])
-@pytest.mark.parametrize("top", [1, 7])
+@pytest.mark.parametrize("rows,V", [(800, 20011), (3000, 2500), (400, 70001)])
+def test_many_rows(lo, rows, V, dtype):
+    x, t, g, ge = make(rows, V, dtype, seed=V)
+    check(lo, x, t, 1.0, 32, g, ge)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [7, 300, 1500, 8000, 40000])
+@pytest.mark.parametrize("top", [1, 7, 32])
 def test_equal_logits_go_by_the_lower_index(lo, V, top, dtype):
+    top = min(top, V)
     x, t, g, ge = make(12, V, dtype, seed=V, std=0.0)             # all equal
     x[1::4] = torch.randint(0, 3, x[1::4].shape, device=DEV).to(dtype)  # three values
     x[2::4, ::2] = -0.0                                              # -0 and +0 are equal
@@ -99,7 +107,7 @@ def test_equal_logits_go_by_the_lower_index(lo, V, top, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("V", [33, 3001, 50257])
+@pytest.mark.parametrize("V", [33, 700, 3001, 14001, 50257])
 def test_tokens_that_are_not_allowed(lo, V, dtype):
     x, t, g, ge = make(10, V, dtype, seed=V)
     x[0] = -INF                     # none allowed
@@ -128,7 +136,7 @@ def test_masked_tokens_at_the_ends_of_the_temperature(lo, V, dtype, tau, weight)
     check(lo, x, t, tau, 3, g, ge * weight)
 
 
-@pytest.mark.parametrize("V", [50, 4000])
+@pytest.mark.parametrize("V", [50, 900, 4000, 60000])
 @pytest.mark.parametrize("bad", [float("nan"), INF])
 def test_spoilt_rows(lo, V, bad):
     x, t, g, ge = make(6, V, torch.float32, seed=2)
@@ -211,7 +219,7 @@ def test_gradient_against_differences(lo):
     assert bool(((want - got).abs() <= 1e-3 * step.norm(dim=-1) * d.norm(dim=-1) + 1e-9).all())
 
 
-@pytest.mark.parametrize("rows,V", [(3, 50257), (200, 3000), (50, 100)])
+@pytest.mark.parametrize("rows,V", [(3, 50257), (200, 3000), (50, 100), (40, 700)])
 def test_captured_and_replayed(lo, rows, V):
     x, t, g, ge = make(rows, V, torch.bfloat16, seed=7)
     stream = torch.cuda.Stream()

@@ -9,12 +9,13 @@
 // gradient reads it once more and writes once. The bound is HBM; per logit the forward issues about six instructions, one of
 // them the exponential, which leaves the SM half idle at the rate BF16 logits arrive.
 //
-// Top alternatives cost nothing per logit: the maximum that every thread keeps for the softmax anyway gives a threshold (the
-// k-th largest of the thread maxima, or a little less) that at least k logits reach. A thread also leaves the maximum of each
-// eighth of its logits; only those that reach the threshold are read again, a percent of a long row, and the few logits that reach
-// it are ranked by counting. (Reading all logits of such threads again cost as much as a fifth of the row: 20 alternatives of
-// 4096 x 131072 BF16 logits 57 us on top of 166.) Order: larger logit first, equal ones by the lower index. A row with more
-// candidates than the lists hold (many equal logits, or fewer allowed tokens than alternatives) falls back to one pass per alternative.
+// Top alternatives cost nothing per logit of a long row: the maximum that every thread keeps for the softmax anyway gives a
+// threshold (the k-th largest of the maxima of 32 groups of threads) that at least k logits reach. A thread also leaves the maximum
+// of each eighth of its logits; only those that reach the threshold are read again, a percent of the row, and the few logits that
+// reach it are ranked by counting. (Reading all logits of such threads again cost as much as a fifth of the row: 20 alternatives of
+// 4096 x 131072 BF16 logits 57 us on top of 166, 21 so.) A row that fits the registers of a few warps is compared with the threshold
+// there. Order: larger logit first, equal ones by the lower index. A row with more candidates than the list holds (many equal logits,
+// or fewer allowed tokens than alternatives) falls back to one pass per alternative.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -40,10 +41,10 @@ constexpr int kUnroll = 4;           // 16-byte loads in flight per thread
 constexpr int kMaxTop = 32;
 constexpr int kSegments = 8;
 constexpr int kMaxCluster = 8;
-constexpr int kWarpRowVocab = 1024;  // rows up to here are handled by one warp each
+constexpr int kWarpRowVocab = 384;   // rows up to here are handled by one warp each
 constexpr int kWarpGradVocab = 256;  // the same in the gradient
-constexpr int kSmallRowVecs = 1024;  // rows of up to so many 16-byte vectors by CTAs of 64 threads
-constexpr int kMiddleRowVecs = 8192; // up to here by 128 threads, longer ones by 256
+constexpr int kSmallRowVecs = 1024;  // gradient: rows of up to so many 16-byte vectors by CTAs of 64 threads, longer ones by 256
+constexpr int kMiddleRowVecs = 8192; // forward: up to so many by 128 threads, longer ones by 256
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLowest = -1e30f;    // x - m is held above this, so that a masked logit contributes 0 * finite
@@ -90,6 +91,19 @@ struct Elem<float> {
         }
         return m;
     }
+    // Bits of a word for kVecsPerWord vectors: set by vector u for the elements that are not below a threshold (a number that T holds).
+    static constexpr int kVecsPerWord = 8;
+    static constexpr float kLowestNumber = -0x1.fffffep127f;
+    static __device__ __forceinline__ uint32_t reach(const uint4& w, float threshold, int u, uint32_t bits) {
+        float x[4];
+        unpack(w, x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (!(x[e] < threshold)) bits |= 1u << (4 * (u % kVecsPerWord) + e);
+        return bits;
+    }
+    static __device__ __forceinline__ int vec_of(int bit) { return bit >> 2; }
+    static __device__ __forceinline__ int element_of(int bit) { return bit & 3; }
     static __device__ __forceinline__ uint4 pack(const float* x) {
         return make_uint4(__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3]));
     }
@@ -126,6 +140,17 @@ struct Elem<__nv_bfloat16> {
         for (int u = 0; u < N; ++u) m = max2(max2(m, max2(w[u].x, w[u].y)), max2(w[u].z, w[u].w));
         return max_nan(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
     }
+    static constexpr int kVecsPerWord = 4;  // (see Elem<float>) the lower elements of the pairs in the lower half
+    static constexpr float kLowestNumber = -0x1.fep127f;
+    static __device__ __forceinline__ uint32_t reach(const uint4& w, float threshold, int u, uint32_t bits) {
+        const __nv_bfloat162 t2 = __float2bfloat162_rn(threshold);
+        const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bits |= ~__hlt2_mask(*reinterpret_cast<const __nv_bfloat162*>(&v[i]), t2) & (0x00010001u << (4 * (u % kVecsPerWord) + i));
+        return bits;
+    }
+    static __device__ __forceinline__ int vec_of(int bit) { return (bit & 15) >> 2; }
+    static __device__ __forceinline__ int element_of(int bit) { return 2 * (bit & 3) + (bit >> 4); }
     static __device__ __forceinline__ uint4 pack(const float* x) {
         uint32_t u[4];
 #pragma unroll
@@ -192,12 +217,6 @@ __device__ __forceinline__ void rebase(Stat& a, float M, float c) {
     a.s *= f;
     a.m = M;
 }
-__device__ __forceinline__ Stat merge(Stat a, Stat b, float c) {
-    const float M = max_nan(a.m, b.m);
-    rebase(a, M, c);
-    rebase(b, M, c);
-    return Stat{M, a.s + b.s, a.t + b.t};
-}
 // What the outputs need of a whole row.
 struct RowStat {
     float m, ln_s, entropy;  // ln_s: of the sum relative to m
@@ -263,47 +282,104 @@ __device__ __forceinline__ void write_row(const FwdArgs& a, int r, const RowStat
     a.logprobs[r] = given ? logprob_of(target_x, st, a.inv_temperature) : 0.f;
 }
 
-// ---------------------------------------------------------------- forward, one CTA (or one cluster of CTAs) per row
-// A threshold that at least `top` (<= 32) and hardly more of the warp's 32 N keys reach: bisection between the smallest of the 32
-// lane maxima (which 32 keys reach) and the largest key. Executed by one warp.
-template <int N>
-__device__ __forceinline__ uint32_t threshold_of(const uint32_t (&k)[N], int top) {
-    uint32_t mine = 0;
+// ---------------------------------------------------------------- alternatives
+// Sorts the warp's keys in descending order (lane 0 the largest).
+__device__ __forceinline__ uint32_t warp_sort(uint32_t x, int lane) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) mine = max(mine, k[i]);
-    uint32_t lo = __reduce_min_sync(0xffffffffu, mine), hi = __reduce_max_sync(0xffffffffu, mine) + 1u;
-    while (hi - lo > 1u) {
-        const uint32_t mid = lo + (hi - lo) / 2u;
-        int n = 0;
+    for (int size = 2; size <= 32; size <<= 1)
 #pragma unroll
-        for (int i = 0; i < N; ++i) n += __popc(__ballot_sync(0xffffffffu, k[i] >= mid));
-        if (n < top) {
-            hi = mid;
-        } else {
-            lo = mid;
-            if (n <= top + 4) break;
+        for (int o = size >> 1; o > 0; o >>= 1) {
+            const uint32_t y = __shfl_xor_sync(0xffffffffu, x, o);
+            const bool larger = ((lane & o) == 0) == ((lane & size) == 0);  // this lane keeps the larger one
+            x = larger ? max(x, y) : min(x, y);
         }
+    return x;
+}
+// The k-th largest of 32 groups' maxima (lane i's key is that of group i): at least k logits of the row reach it, and where the large ones
+// are spread evenly -32 ln(1 - k / 32) do in the mean (31 for 20 alternatives), however long the row. Never -inf: a masked logit is
+// only an alternative where fewer tokens are allowed than alternatives asked for, which is left to write_alternatives' last resort.
+template <typename T>
+__device__ __forceinline__ float threshold_of(uint32_t group, int top, int lane) {
+    return from_key(max(__shfl_sync(0xffffffffu, warp_sort(group, lane), top - 1), to_key(Elem<T>::kLowestNumber)));
+}
+__device__ __forceinline__ void write_alternative(const FwdArgs& a, int r, const RowStat& total, int rank, uint64_t y) {
+    a.top_logprobs[(long long)r * a.top + rank] = logprob_of(from_key(uint32_t(y >> 32)), total, a.inv_temperature);
+    a.top_tokens[(long long)r * a.top + rank] = index_of(y);
+}
+// Ranks the n candidates of a row, whose indices are in `cand`, by counting: the threads of a row (one warp or a whole CTA). Where they are
+// fewer than alternatives or more than the list holds: one pass over the row per alternative, the best logit below the one before.
+template <typename T, int kThreads, int kList>
+__device__ __forceinline__ void write_alternatives(const FwdArgs& a, int r, const RowStat& total, const T* row, const RowSplit& sp, int tid, int n, uint64_t* cand,
+                                                   uint64_t* s_best) {
+    const int lane = tid & 31, warp = tid >> 5;
+    if (n >= a.top && n <= kList) {
+        const bool few = kThreads == 32 || n <= 64;  // one warp's work
+        if (few && warp > 0) return;
+        const int step = few ? 32 : kThreads;
+        for (int i = tid; i < n; i += step) {
+            const int index = int(cand[i]);
+            cand[i] = candidate(to_key(Elem<T>::load(row + index)), index);
+        }
+        if (few) __syncwarp();
+        else __syncthreads();
+        for (int i = tid; i < n; i += step) {
+            const uint64_t y = cand[i];
+            int rank = 0;
+            for (int j = 0; j < n; ++j) rank += cand[j] > y;
+            if (rank < a.top) write_alternative(a, r, total, rank, y);
+        }
+        return;
     }
-    return lo;
+    const uint4* vec = reinterpret_cast<const uint4*>(row + sp.head);
+    const int singles = sp.head + sp.tail;
+    uint64_t before = ~uint64_t(0);
+    for (int k = 0; k < a.top; ++k) {
+        uint64_t best = 0;
+        auto see = [&](float x, int index) {
+            const uint64_t y = candidate(to_key(x), index);
+            if (y < before && y > best) best = y;
+        };
+        for (int i = tid; i < sp.vecs; i += kThreads) {
+            constexpr int E = Elem<T>::kPerVec;
+            float x[E];
+            Elem<T>::unpack(__ldg(vec + i), x);
+#pragma unroll
+            for (int e = 0; e < E; ++e) see(x[e], sp.head + i * E + e);
+        }
+        if (tid < singles) {
+            const int index = tid < sp.head ? tid : a.V - singles + tid;
+            see(Elem<T>::load(row + index), index);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) {
+            const uint64_t y = __shfl_xor_sync(0xffffffffu, best, o);
+            if (y > best) best = y;
+        }
+        if constexpr (kThreads > 32) {
+            __syncthreads();  // the round before has been read
+            if (lane == 0) s_best[warp] = best;
+            __syncthreads();
+            for (int i = 0; i < kThreads / 32; ++i) best = s_best[i] > best ? s_best[i] : best;
+        }
+        if (tid == 0) write_alternative(a, r, total, k, best);
+        before = best;
+    }
 }
 
-template <typename T, int kThreads>
+// ---------------------------------------------------------------- forward, one CTA (or one cluster of CTAs) per row
+template <typename T, int kThreads, bool CLUSTER>
 __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const FwdArgs a) {
     constexpr int E = Elem<T>::kPerVec, kWarps = kThreads / 32, kMaxCand = kThreads >= 256 ? 1024 : 256, kMaxHot = kThreads >= 256 ? 256 : 128;
-    __shared__ float s_max[kWarps], s_sum[kWarps], s_sum_a[kWarps], s_part_max;
-    __shared__ Stat s_part, s_total;  // of this CTA's part of the row, and of the row
-    __shared__ uint32_t s_key[kThreads];
-    __shared__ uint64_t s_cand[kMaxCand];
-    __shared__ uint64_t s_sel[kMaxTop];
-    __shared__ uint64_t s_best[kWarps];
+    __shared__ float s_max[kWarps], s_sum[kWarps * kMaxCluster], s_sum_a[kWarps * kMaxCluster], s_part_max[kMaxCluster];
+    __shared__ uint32_t s_key[kThreads], s_part_key[kMaxCluster][32];
+    __shared__ uint64_t s_cand[kMaxCand], s_best[kWarps];
     __shared__ float s_segment[kSegments][kThreads];
     __shared__ int s_hot[kMaxHot];  // segments that hold a candidate: thread + kThreads * segment
     __shared__ int s_nhot, s_ncand;
-    __shared__ uint32_t s_threshold;
 
     pdl_launch_dependents();
     const cg::cluster_group cluster = cg::this_cluster();
-    const int parts = int(cluster.num_blocks()), part = int(cluster.block_rank());
+    const int parts = CLUSTER ? int(cluster.num_blocks()) : 1, part = CLUSTER ? int(cluster.block_rank()) : 0;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const float c = a.inv_temperature * kLog2e;
     const Pair c2 = pair(c, c);
@@ -386,197 +462,246 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const FwdArgs 
                 if (i0 + u * kThreads + warp * 32 < end) add_vec(w[u]);
         }
     }
-    const float target_x = given && tid == 0 ? Elem<T>::load(row + target) : 0.f;  // under way with the reductions
+    const float target_x = given && tid == 0 && part == 0 ? Elem<T>::load(row + target) : 0.f;  // under way with the reductions
     {
         float sa, sb, ta, tb;
         split(s2, sa, sb), split(t2, ta, tb);
         st.s = sa + sb, st.t = ta + tb;
     }
-    const float warp_max = warp_max_nan(my_max);
-    if (lane == 0) s_max[warp] = warp_max;
+    auto barrier = [&]() {
+        if constexpr (CLUSTER) cluster.sync();
+        else __syncthreads();
+    };
+    float row_max = warp_max_nan(my_max);
+    if (lane == 0) s_max[warp] = row_max;
     s_key[tid] = to_key(my_max);
     if (tid == 0) s_nhot = 0, s_ncand = 0;
-    __syncthreads();
-    float part_max = s_max[0];
+    barrier();
+    uint32_t group = 0u;  // the largest key of the row's threads with this lane
+    if constexpr (CLUSTER) {  // a warp fetches what a CTA of the row has
+        for (int p = warp; p < parts; p += kWarps) {
+            const float* from = cluster.map_shared_rank(s_max, p);
+            const uint32_t* keys = cluster.map_shared_rank(s_key, p);
+            const float x = warp_max_nan(lane < kWarps ? from[lane] : -INFINITY);
+            uint32_t k = 0u;
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) part_max = max_nan(part_max, s_max[w]);
-    rebase(st, max_nan(part_max, kFloor), c);
-    if (edge >= 0) {
-        const float x = (max_nan(edge_x, kFloor) - st.m) * c, e = ex2(x);
-        st.s += e, st.t = fmaf(e, x, st.t);
-    }
-    const float warp_s = warp_add(st.s), warp_t = warp_add(st.t);
-    if (lane == 0) s_sum[warp] = warp_s, s_sum_a[warp] = warp_t;
-    if (a.top > 0 && warp == kWarps - 1) {
-        uint32_t k[kWarps];
+            for (int i = 0; i < kWarps; ++i) k = max(k, keys[i * 32 + lane]);
+            s_part_key[p][lane] = k;
+            if (lane == 0) s_part_max[p] = x;
+        }
+        __syncthreads();
+        for (int p = 0; p < parts; ++p) row_max = max_nan(row_max, s_part_max[p]), group = max(group, s_part_key[p][lane]);
+    } else {
 #pragma unroll
-        for (int i = 0; i < kWarps; ++i) k[i] = s_key[i * 32 + lane];
-        const uint32_t threshold = threshold_of(k, a.top);
-        if (lane == 0) s_threshold = threshold;
+        for (int i = 0; i < kWarps; ++i) row_max = max_nan(row_max, s_max[i]), group = max(group, s_key[i * 32 + lane]);
     }
-    __syncthreads();
-    if (tid == 0) {
-        Stat x{max_nan(part_max, kFloor), 0.f, 0.f};
+    float s = 0.f, t = 0.f;
+    if (fabsf(row_max) < kWild) {
+        rebase(st, row_max, c);
+        s = st.s, t = st.t;
+        if (edge >= 0) add_exact(edge_x, row_max, c, s, t);
+    } else if (row_max != -INFINITY) {  // (see Stat)
+        for (int i = begin + tid; i < end; i += kThreads) {
+            float x[E];
+            Elem<T>::unpack(__ldg(vec + i), x);
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) x.s += s_sum[w], x.t += s_sum_a[w];
-        s_part = x, s_part_max = part_max;
+            for (int e = 0; e < E; ++e) add_exact(x[e], row_max, c, s, t);
+        }
+        if (edge >= 0) add_exact(edge_x, row_max, c, s, t);
     }
-
+    s = warp_add(s), t = warp_add(t);
+    // what follows goes to the first CTA of the row
+    float *sums = s_sum, *sums_a = s_sum_a;
+    int* ncand = &s_ncand;
+    uint64_t* cand = s_cand;
+    if constexpr (CLUSTER) {
+        sums = cluster.map_shared_rank(s_sum, 0) + part * kWarps, sums_a = cluster.map_shared_rank(s_sum_a, 0) + part * kWarps;
+        ncand = cluster.map_shared_rank(&s_ncand, 0), cand = cluster.map_shared_rank(s_cand, 0);
+    }
+    if (lane == 0) sums[warp] = s, sums_a[warp] = t;
     if (a.top > 0) {
-        // a masked logit is only ever an alternative where fewer tokens are allowed than alternatives asked for: the fallback
-        const uint32_t threshold = max(s_threshold, kKeyNegInf + 1u);
-        if (s_key[tid] >= threshold)
+        const float threshold = threshold_of<T>(group, a.top, lane);
+        if (!(my_max < threshold))
             for (int i = 0; i < segment; ++i)  // its own: no other thread has written them
-                if (to_key(s_segment[i][tid]) >= threshold) {
+                if (!(s_segment[i][tid] < threshold)) {
                     const int at = atomicAdd(&s_nhot, 1);
                     if (at < kMaxHot) s_hot[at] = tid + kThreads * i;
                 }
         __syncthreads();
         const int nhot = s_nhot;
-        auto consider = [&](float x, int index) {
-            const uint32_t key = to_key(x);
-            if (key < threshold) return;
-            const int at = atomicAdd(&s_ncand, 1);
-            if (at < kMaxCand) s_cand[at] = candidate(key, index);
-        };
         // every (segment, vector of it) to a thread of its own, several at a time, so that the reads are under way together
         const int per = per_segment * kUnroll, pairs = nhot <= kMaxHot ? nhot * per : 0;
+        auto vec_at = [&](int i) {
+            const int hot = s_hot[i / per];
+            return begin + hot % kThreads + ((hot / kThreads) * per + i % per) * kThreads;
+        };
         for (int i0 = tid; i0 < pairs; i0 += kThreads * kUnroll) {
             uint4 w[kUnroll];
-            int at[kUnroll];
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u) {
-                const int i = i0 + u * kThreads;
-                at[u] = end;
-                if (i < pairs) {
-                    const int hot = s_hot[i / per];
-                    at[u] = begin + hot % kThreads + ((hot / kThreads) * per + i % per) * kThreads;
-                }
-                w[u] = at[u] < end ? __ldg(vec + at[u]) : nothing;
+                const int i = i0 + u * kThreads, at = i < pairs ? vec_at(i) : end;
+                w[u] = at < end ? __ldg(vec + at) : nothing;
             }
+            static_assert(kUnroll <= Elem<T>::kVecsPerWord, "");
+            uint32_t bits = 0u;
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u) {
-                const uint4 one[1] = {w[u]};
-                if (to_key(Elem<T>::largest(one)) < threshold) continue;
-                float x[E];
-                Elem<T>::unpack(w[u], x);
-#pragma unroll
-                for (int e = 0; e < E; ++e) consider(x[e], head + at[u] * E + e);
+            for (int u = 0; u < kUnroll; ++u) bits = Elem<T>::reach(w[u], threshold, u, bits);
+            if (bits != 0u) {
+                int at = atomicAdd(ncand, __popc(bits));
+                for (; bits != 0u && at < kMaxCand; bits &= bits - 1u, ++at) {
+                    const int bit = __ffs(bits) - 1;
+                    cand[at] = head + vec_at(i0 + Elem<T>::vec_of(bit) * kThreads) * E + Elem<T>::element_of(bit);
+                }
             }
         }
-        if (edge >= 0) consider(edge_x, edge);
-        __syncthreads();
-        const int n = s_ncand;
-        if (n >= a.top && n <= kMaxCand && nhot <= kMaxHot) {
-            for (int i = tid; i < n; i += kThreads) {
-                const uint64_t mine = s_cand[i];
-                int rank = 0;
-                for (int j = 0; j < n; ++j) rank += s_cand[j] > mine;
-                if (rank < a.top) s_sel[rank] = mine;
-            }
-        } else {
-            // one pass per alternative: the best candidate below the one before. A part of a row (of a cluster) may run out.
-            uint64_t before = ~uint64_t(0);
-            for (int k = 0; k < a.top; ++k) {
-                uint64_t best = 0;
-                for (int i = begin + tid; i < end; i += kThreads) {
-                    float x[E];
-                    Elem<T>::unpack(__ldg(vec + i), x);
-#pragma unroll
-                    for (int e = 0; e < E; ++e) {
-                        const uint64_t y = candidate(to_key(x[e]), head + i * E + e);
-                        if (y < before && y > best) best = y;
-                    }
-                }
-                if (edge >= 0) {
-                    const uint64_t y = candidate(to_key(edge_x), edge);
-                    if (y < before && y > best) best = y;
-                }
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) {
-                    const uint64_t y = __shfl_xor_sync(0xffffffffu, best, o);
-                    if (y > best) best = y;
-                }
-                __syncthreads();  // the previous round's s_best has been read
-                if (lane == 0) s_best[warp] = best;
-                __syncthreads();
-                for (int i = 0; i < kWarps; ++i) best = s_best[i] > best ? s_best[i] : best;
-                if (tid == 0) s_sel[k] = best;
-                before = best;
-            }
+        if (edge >= 0 && !(edge_x < threshold)) {
+            const int at = atomicAdd(ncand, 1);
+            if (at < kMaxCand) cand[at] = edge;
         }
+        if (nhot > kMaxHot && tid == 0) atomicAdd(ncand, kMaxCand + 1);  // not looked for
     }
-
-    // the row's maximum, and whether it has to be summed again (every CTA of the row comes to the same answer)
-    float row_max = part_max;
-    if (parts > 1) {
-        cluster.sync();
-        for (int p = 0; p < parts; ++p) row_max = max_nan(row_max, *cluster.map_shared_rank(&s_part_max, p));
-    }
-    const bool wild = !(fabsf(row_max) < kWild);
-    if (wild) {
-        float s = 0.f, t = 0.f;
-        if (row_max != -INFINITY) {
-            for (int i = begin + tid; i < end; i += kThreads) {
-                float x[E];
-                Elem<T>::unpack(__ldg(vec + i), x);
-#pragma unroll
-                for (int e = 0; e < E; ++e) add_exact(x[e], row_max, c, s, t);
-            }
-            if (edge >= 0) add_exact(edge_x, row_max, c, s, t);
-        }
-        s = warp_add(s), t = warp_add(t);
-        __syncthreads();  // s_sum has been read
-        if (lane == 0) s_sum[warp] = s, s_sum_a[warp] = t;
-        __syncthreads();
-        if (tid == 0) {
-            for (int w = 1; w < kWarps; ++w) s += s_sum[w], t += s_sum_a[w];
-            s_part = Stat{row_max, s, t};
-        }
-    }
-    if (parts > 1) {  // rank 0 joins what the CTAs of the row found
-        cluster.sync();
-        if (part == 0) {
-            if (tid == 0) {
-                Stat x = s_part;
-                for (int p = 1; p < parts; ++p) {
-                    const Stat y = *cluster.map_shared_rank(&s_part, p);
-                    x = wild ? Stat{row_max, x.s + y.s, x.t + y.t} : merge(x, y, c);
-                }
-                s_total = x;
-            }
-            const int n = parts * a.top;
-            for (int i = tid; i < n; i += kThreads) s_cand[i] = cluster.map_shared_rank(s_sel, i / a.top)[i % a.top];
-        }
-        cluster.sync();  // the other CTAs' shared memory has been read
-        if (part != 0) return;
-        const int n = parts * a.top;
-        for (int i = tid; i < n; i += kThreads) {
-            const uint64_t mine = s_cand[i];
-            int rank = 0;
-            for (int j = 0; j < n; ++j) rank += s_cand[j] > mine;
-            if (mine != 0 && rank < a.top) s_sel[rank] = mine;
-        }
-    } else if (tid == 0) {
-        s_total = s_part;
-    }
-    __syncthreads();
-    const RowStat total = finish(s_total);
+    barrier();
+    if (part != 0) return;
+    s = t = 0.f;
+    for (int i = 0; i < parts * kWarps; ++i) s += s_sum[i], t += s_sum_a[i];
+    const RowStat total = finish(Stat{row_max, s, t});
     if (tid == 0) write_row(a, r, total, given, target_x);
-    if (tid < a.top) {
-        const uint64_t y = s_sel[tid];
-        a.top_logprobs[(long long)r * a.top + tid] = logprob_of(from_key(uint32_t(y >> 32)), total, a.inv_temperature);
-        a.top_tokens[(long long)r * a.top + tid] = index_of(y);
+    if (a.top > 0) write_alternatives<T, kThreads, kMaxCand>(a, r, total, row, sp, tid, s_ncand, s_cand, s_best);
+}
+
+// ---------------------------------------------------------------- forward, rows that fit the registers of a few warps
+// kWarps warps to a row (kWarps = 1: four rows to a CTA), N vectors per thread, all loads of a row under way together. With the row in
+// registers its maximum is known before the sums, which are then exact in one go, and the alternatives are compared in place: 32
+// groups of threads give a threshold (the k-th largest of their maxima) that a few dozen logits of the row reach. Two barriers.
+template <typename T, int kWarps, int N>
+__global__ void __launch_bounds__(kWarps == 1 ? 128 : 32 * kWarps) token_logprobs_resident_kernel(const FwdArgs a) {
+    constexpr int E = Elem<T>::kPerVec, kThreads = 32 * kWarps, kRows = kWarps == 1 ? 4 : 1, kList = 256;
+    __shared__ uint64_t s_cand[kRows][kList];
+    __shared__ int s_ncand[kRows];
+    __shared__ float s_max[kWarps], s_sum[kWarps], s_sum_a[kWarps];
+    __shared__ uint32_t s_key[kWarps][32];
+    __shared__ uint64_t s_best[kWarps];
+    pdl_launch_dependents();
+    const int lane = threadIdx.x & 31, local = kWarps == 1 ? threadIdx.x >> 5 : 0, warp = kWarps == 1 ? 0 : threadIdx.x >> 5;
+    const int tid = warp * 32 + lane;
+    auto barrier = [&]() {
+        if constexpr (kWarps == 1) __syncwarp();
+        else __syncthreads();
+    };
+    const long long r64 = (long long)blockIdx.x * kRows + local;
+    const float c = a.inv_temperature * kLog2e;
+    const uint4 nothing = make_uint4(Elem<T>::kNegInf, Elem<T>::kNegInf, Elem<T>::kNegInf, Elem<T>::kNegInf);
+    pdl_wait();
+    if (r64 >= a.rows) return;
+    const int r = int(r64);
+    const T* row = static_cast<const T*>(a.logits) + a.row_stride * r;
+    const RowSplit sp = split_row(row, a.V);
+    const int head = sp.head;
+    const uint4* vec = reinterpret_cast<const uint4*>(row + head);
+    uint4 w[N];
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+        const int i = u * kThreads + tid;
+        w[u] = i < sp.vecs ? __ldg(vec + i) : nothing;
     }
+    // the single element in front of or behind the vectors that this thread owns, if any
+    const int edge = tid < head ? tid : (tid >= 16 && tid < 16 + sp.tail) ? head + sp.vecs * E + (tid - 16) : -1;
+    const float edge_x = edge >= 0 ? Elem<T>::load(row + edge) : -INFINITY;
+    const int target = a.targets[r];
+    const bool given = (unsigned)target < (unsigned)a.V;
+    const float target_x = given && tid == 0 ? Elem<T>::load(row + target) : 0.f;
+
+    const float my_max = max_nan(Elem<T>::largest(w), edge_x);
+    float m = warp_max_nan(my_max);
+    uint32_t group = to_key(my_max);
+    if (tid == 0) s_ncand[local] = 0;
+    if constexpr (kWarps > 1) {
+        if (lane == 0) s_max[warp] = m;
+        s_key[warp][lane] = group;
+    }
+    barrier();
+    if constexpr (kWarps > 1) {
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) m = max_nan(m, s_max[i]), group = max(group, s_key[i][lane]);
+    }
+    float s = 0.f, t = 0.f;
+    if (fabsf(m) < kWild) {  // (see Stat)
+        const Pair c2 = pair(c, c), neg_m = pair(-m, -m);
+        Pair s2 = pair(0.f, 0.f), t2 = pair(0.f, 0.f);
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            if (u * kThreads + warp * 32 >= sp.vecs) break;
+            float x[E];
+            Elem<T>::unpack(Elem<T>::raise(w[u]), x);
+#pragma unroll
+            for (int e = 0; e < E; e += 2) {
+                float a0, a1;
+                const Pair arg = mul(add(pair(x[e], x[e + 1]), neg_m), c2);
+                split(arg, a0, a1);
+                const Pair ex = pair(ex2(a0), ex2(a1));
+                s2 = add(s2, ex);
+                t2 = fma(ex, arg, t2);
+            }
+        }
+        float sb, tb;
+        split(s2, s, sb), split(t2, t, tb);
+        s += sb, t += tb;
+        if (edge >= 0) add_exact(edge_x, m, c, s, t);
+    } else if (m != -INFINITY) {  // read again: the elements of the row as numbers are not kept beside their words
+        for (int i = tid; i < sp.vecs; i += kThreads) {
+            float x[E];
+            Elem<T>::unpack(__ldg(vec + i), x);
+#pragma unroll
+            for (int e = 0; e < E; ++e) add_exact(x[e], m, c, s, t);
+        }
+        if (edge >= 0) add_exact(edge_x, m, c, s, t);
+    }
+    s = warp_add(s), t = warp_add(t);
+    if constexpr (kWarps > 1) {
+        if (lane == 0) s_sum[warp] = s, s_sum_a[warp] = t;
+    }
+    if (a.top > 0) {
+        const float threshold = threshold_of<T>(group, a.top, lane);
+        constexpr int kPer = Elem<T>::kVecsPerWord, kWords = (N + kPer - 1) / kPer;
+        uint32_t bits[kWords];
+        int count = edge >= 0 && !(edge_x < threshold);
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            bits[i] = 0u;
+#pragma unroll
+            for (int u = i * kPer; u < min(N, (i + 1) * kPer); ++u) bits[i] = Elem<T>::reach(w[u], threshold, u, bits[i]);
+            count += __popc(bits[i]);
+        }
+        if (count > 0) {
+            int at = atomicAdd(&s_ncand[local], count);
+            if (at + count <= kList) {
+                if (edge >= 0 && !(edge_x < threshold)) s_cand[local][at++] = edge;
+#pragma unroll
+                for (int i = 0; i < kWords; ++i)
+                    for (uint32_t left = bits[i]; left != 0u; left &= left - 1u) {
+                        const int bit = __ffs(left) - 1;
+                        s_cand[local][at++] = head + ((i * kPer + Elem<T>::vec_of(bit)) * kThreads + tid) * E + Elem<T>::element_of(bit);
+                    }
+            }
+        }
+    }
+    barrier();
+    if constexpr (kWarps > 1) {
+        s = t = 0.f;
+#pragma unroll
+        for (int i = 0; i < kWarps; ++i) s += s_sum[i], t += s_sum_a[i];
+    }
+    const RowStat total = finish(Stat{m, s, t});
+    if (tid == 0) write_row(a, r, total, given, target_x);
+    if (a.top > 0) write_alternatives<T, kThreads, kList>(a, r, total, row, sp, tid, s_ncand[local], s_cand[local], s_best);
 }
 
 // ---------------------------------------------------------------- forward, one warp per (short) row
 // N: elements per lane, all of them in registers.
 template <typename T, int N>
 __global__ void __launch_bounds__(kWarpRowThreads) token_logprobs_warp_kernel(const FwdArgs a) {
-    constexpr int kWarps = kWarpRowThreads / 32, kList = 128;
-    __shared__ uint64_t s_cand[kWarps][kList];
-    __shared__ int s_ncand[kWarps];
+    constexpr int kWarps = kWarpRowThreads / 32;
+    __shared__ uint64_t s_cand[kWarps][32 * N];
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const long long r64 = (long long)blockIdx.x * kWarps + warp;
@@ -604,50 +729,24 @@ __global__ void __launch_bounds__(kWarpRowThreads) token_logprobs_warp_kernel(co
     if (lane == 0) write_row(a, r, total, given, target_x);
     if (a.top == 0) return;
 
-    // alternatives: as above, with the lane maxima; rows too short for 32 lanes have threshold 0 (every logit is a candidate)
-    const uint32_t k[1] = {lane < a.V ? to_key(mine) : 0u};
-    const uint32_t threshold = threshold_of(k, a.top);
-    if (lane == 0) s_ncand[warp] = 0;
-    __syncwarp();
+    // alternatives: as above, with the lanes as groups; a row too short for 32 of them, or with too few allowed tokens, has the threshold
+    // -inf (every logit is a candidate). The list holds them all.
+    const uint32_t group = lane < a.V ? to_key(mine) : 0u;
+    const float threshold = from_key(max(__shfl_sync(0xffffffffu, warp_sort(group, lane), a.top - 1), kKeyNegInf));
+    int n = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const int v = i * 32 + lane;
-        const uint32_t key = to_key(x[i]);
-        if (v < a.V && key >= threshold) {
-            const int at = atomicAdd(&s_ncand[warp], 1);
-            if (at < kList) s_cand[warp][at] = candidate(key, v);
-        }
+        const bool reaches = i * 32 + lane < a.V && !(x[i] < threshold);
+        const uint32_t who = __ballot_sync(0xffffffffu, reaches);
+        if (reaches) s_cand[warp][n + __popc(who & ((1u << lane) - 1u))] = candidate(to_key(x[i]), i * 32 + lane);
+        n += __popc(who);
     }
     __syncwarp();
-    const int n = s_ncand[warp];
-    auto write = [&](int rank, uint64_t y) {
-        a.top_logprobs[(long long)r * a.top + rank] = logprob_of(from_key(uint32_t(y >> 32)), total, a.inv_temperature);
-        a.top_tokens[(long long)r * a.top + rank] = index_of(y);
-    };
-    if (n <= kList) {
-        for (int i = lane; i < n; i += 32) {
-            const uint64_t y = s_cand[warp][i];
-            int rank = 0;
-            for (int j = 0; j < n; ++j) rank += s_cand[warp][j] > y;
-            if (rank < a.top) write(rank, y);
-        }
-        return;
-    }
-    uint64_t before = ~uint64_t(0);
-    for (int i = 0; i < a.top; ++i) {
-        uint64_t best = 0;
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const uint64_t y = candidate(to_key(x[j]), j * 32 + lane);
-            if (j * 32 + lane < a.V && y < before && y > best) best = y;
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-            const uint64_t y = __shfl_xor_sync(0xffffffffu, best, o);
-            if (y > best) best = y;
-        }
-        if (lane == 0) write(i, best);
-        before = best;
+    for (int i = lane; i < n; i += 32) {
+        const uint64_t y = s_cand[warp][i];
+        int rank = 0;
+        for (int j = 0; j < n; ++j) rank += s_cand[warp][j] > y;
+        if (rank < a.top) write_alternative(a, r, total, rank, y);
     }
 }
 
@@ -799,22 +898,39 @@ cudaError_t launch_rows(const FwdArgs& a, cudaStream_t stream) {
     // full round of loads.
     int parts = 1;
     while (parts < kMaxCluster && (long long)a.rows * parts * 2 <= 296 && a.V / (parts * 2) >= kThreads * Elem<T>::kPerVec) parts *= 2;
-    return launch_pdl_cluster(token_logprobs_kernel<T, kThreads>, dim3(unsigned(a.rows) * unsigned(parts)), dim3(unsigned(parts)), dim3(kThreads), 0, stream, a);
+    if (parts == 1) return launch_pdl(token_logprobs_kernel<T, kThreads, false>, dim3(unsigned(a.rows)), dim3(kThreads), 0, stream, a);
+    return launch_pdl_cluster(token_logprobs_kernel<T, kThreads, true>, dim3(unsigned(a.rows) * unsigned(parts)), dim3(unsigned(parts)), dim3(kThreads), 0, stream, a);
 }
 
+template <typename T, int kWarps, int N>
+cudaError_t launch_resident(const FwdArgs& a, cudaStream_t stream) {
+    constexpr int rows = kWarps == 1 ? 4 : 1, threads = kWarps == 1 ? 128 : 32 * kWarps;
+    return launch_pdl(token_logprobs_resident_kernel<T, kWarps, N>, dim3((a.rows + rows - 1) / rows), dim3(threads), 0, stream, a);
+}
 template <typename T>
 cudaError_t launch_forward(const FwdArgs& a, cudaStream_t stream) {
     if (a.V <= kWarpRowVocab) {
         constexpr int rows = kWarpRowThreads / 32;
-        auto kern = a.V <= 128 ? token_logprobs_warp_kernel<T, 4> : a.V <= 384 ? token_logprobs_warp_kernel<T, 12> : token_logprobs_warp_kernel<T, 32>;
+        auto kern = a.V <= 128 ? token_logprobs_warp_kernel<T, 4> : token_logprobs_warp_kernel<T, 12>;
         return launch_pdl(kern, dim3((a.rows + rows - 1) / rows), dim3(kWarpRowThreads), 0, stream, a);
     }
-    // A thread should have some rounds of its row, and the ends of rows should not fall together on an SM: the shorter the row, the
-    // smaller (and the more) the CTAs. Measured with 64 / 128 / 256 threads, BF16, without and with 20 alternatives: 8192 x 6000
-    // 30 / 43 / - us, 4096 x 12000 25 and 42 / 21 and 36 / 29 and 51 us, 6001 x 50304 - / 98 and 121 / 104 and 137 us, 4096 x 131072 - / 195
-    // and 255 / 164 and 186 us.
+    // Rows that fit the registers of a few warps: as few warps as hold them. Measured without and with 20 alternatives, here and by the
+    // kernel for long rows: BF16 16384 x 2001 14 and 27 us (34 and 86), 8388 x 4000 14 and 26 (23 and 52), 4096 x 8192 14 and 21 (17 and 33),
+    // 2097 x 16000 14 and 21 (15 and 23); FP32 5592 x 6000 23 and 38 (27 and 42); one row of 8192 2.3 and 3.7 us (4.0 and 7).
     const int vecs = a.V / Elem<T>::kPerVec;
-    return vecs <= kSmallRowVecs ? launch_rows<T, 64>(a, stream) : vecs <= kMiddleRowVecs ? launch_rows<T, 128>(a, stream) : launch_rows<T, 256>(a, stream);
+    if (vecs <= 128) return launch_resident<T, 1, 4>(a, stream);
+    if (vecs <= 256) return launch_resident<T, 1, 8>(a, stream);
+    if (vecs <= 512) return launch_resident<T, 2, 8>(a, stream);
+    if (vecs <= 1024) return launch_resident<T, 4, 8>(a, stream);
+    if (vecs <= 2048) return launch_resident<T, 4, 16>(a, stream);
+    // Eight warps with 100 registers are two CTAs to an SM, which wait for their loads together: up to two rounds of them (BF16
+    // 300 x 32000 7.1 and 10.5 us, 8.2 and 11.6 by the kernel below; 1118 x 30000 15.7 and 24.7, 14.6 and 20.2 below).
+    if (vecs <= 4096 && a.rows <= 4 * 148) return launch_resident<T, 8, 16>(a, stream);
+    // A thread should have some rounds of its row, and the ends of rows should not fall together on an SM: the shorter the row, the
+    // smaller (and the more) the CTAs, unless there are too few rows to fill the card with small ones (and too many for clusters of them).
+    // Measured with 128 / 256 threads, BF16, without and with 20 alternatives: 3355 x 20000 28 and 39 / 34 and 51 us, 6001 x 50304 98
+    // and 121 / 104 and 137 us, 64 x 32000 4.6 and 7.9 / 5.3 and 8.2 us, 600 x 50257 18 and 24 / 15 and 21 us, 671 x 100000 40 and 46 / 31 and 35 us.
+    return vecs <= kMiddleRowVecs && (a.rows > 5 * 148 || a.rows <= 148) ? launch_rows<T, 128>(a, stream) : launch_rows<T, 256>(a, stream);
 }
 
 template <typename T, int kThreads>
