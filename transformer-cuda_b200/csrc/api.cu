@@ -987,7 +987,7 @@ extern "C" int b200attn_bwd_bf16_ragged(const void* q, const void* k, const void
 // ---------------------------------------------------------------------- one new token per sequence
 extern "C" long long b200attn_decode_workspace_bytes(int B, int T, int H, int Hkv, int d) {
     if (B <= 0 || T <= 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || d <= 0) return 0;
-    const int splits = decode_splits(B, T, H, Hkv);
+    const int splits = decode_splits(B, T, H, Hkv, d);
     return decode_needs_workspace(splits) ? (long long)B * H * splits * (d + 2) * (long long)sizeof(float) : 0;
 }
 
@@ -1028,7 +1028,7 @@ extern "C" int b200attn_decode_bf16(const void* q, const void* k_cache, const vo
     a.k_batch = k_batch_stride, a.k_row = k_row_stride, a.k_head = k_head_stride;
     a.v_batch = v_batch_stride, a.v_row = v_row_stride, a.v_head = v_head_stride;
     a.scale = scale;
-    a.splits = T > 0 ? decode_splits(B, T, H, Hkv) : 1;
+    a.splits = T > 0 ? decode_splits(B, T, H, Hkv, d) : 1;
     if (need > 0) {
         a.part_o = static_cast<float*>(workspace);
         a.part_ml = a.part_o + (long long)B * H * a.splits * d;

@@ -32,6 +32,7 @@ constexpr int kThreads = 32 * kWarps;
 constexpr int kTile = 16;                      // keys per warp and step
 constexpr int kStages = 3;                     // steps of K and V in flight per warp
 constexpr int kRound = kTile * kWarps;         // keys of a CTA and step; a split is a multiple of it
+constexpr int kLeastPart = 2 * kRound;         // keys of a split at least: fewer cost more to set up and to join than to read
 constexpr int kMaxCluster = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -56,7 +57,7 @@ __device__ __forceinline__ void copy_wait() {
 // Keys of one split of a sequence of `len` keys (the last one may be shorter; splits past the end are empty).
 __device__ __forceinline__ int chunk_of(int len, int splits) {
     const int c = (len + splits - 1) / splits;
-    return max(1, (c + kRound - 1) / kRound) * kRound;
+    return max(kLeastPart, (c + kRound - 1) / kRound * kRound);
 }
 __device__ __forceinline__ int length_of(const DecodeArgs& a, int b) { return min(max(a.lengths[b], 0), a.T); }
 
@@ -378,14 +379,23 @@ cudaError_t launch(const DecodeArgs& a, cudaStream_t stream) {
 }  // namespace
 
 bool decode_needs_workspace(int splits) { return splits > kMaxCluster; }
-int decode_splits(int B, int T, int H, int Hkv) {
+int decode_splits(int B, int T, int H, int Hkv, int d) {
     const int G = H / Hkv, R = G <= 8 ? 8 : 16;
     const long long items = (long long)B * Hkv * ((G + R - 1) / R);
-    // Six CTAs per SM, three rounds of the two that fit: sequences differ in length, and parts of one long sequence end together
-    // (measured, 1 / 1.5 / 2 / 3 / 8 rounds: 64 sequences up to 4096 keys 74 / 73 / 72 / 72 / 72 us, 8 of 8192 keys 59 / 50 / 53 / 49 / 51 us,
-    // one of 109,000 keys 75 / 78 / 77 / 80 / 82 us). A part has at least two steps.
-    long long splits = (148 * 6 + items - 1) / items;
-    const long long most = (T + 2 * kRound - 1) / (2 * kRound);
+    // What a CTA costs beside its keys (some 4 us from launch to join) is paid once per round of the CTAs that the card holds, so: one
+    // round, or as many full ones as it takes for a split of the longest sequence the cache can hold to have no more than 1280 keys
+    // (768 of 64 dims), up to four; sequences differ in length, and short splits even that out. One sequence alone needs no evening
+    // out. Measured against six CTAs per SM whatever the lengths (us, that / this): 65 sequences up to 392 keys, 8 key heads, d 128 20.5 /
+    // 11.5, 86 up to 989, 1 key head 17.7 / 8.5, 47 up to 1166, 4 key heads 30 / 19, 64 up to 4096, 8 key heads 69 / 69, one of 131,000
+    // 76.7 / 73.6 (a round and a part of the next: 79.6), 16 up to 16384, 4 key heads, d 64 21.8 / 20.8; 18 up to 4035, 4 key heads, d 128
+    // the other way: 16.0 / 18.8.
+    const long long resident = (d == 64 ? 4 : 2) * 148, keys = d == 64 ? 768 : 1280, alone = resident / items > 1 ? resident / items : 1;
+    long long want = (T + keys - 1) / keys;
+    if (want > 4 * resident / items) want = 4 * resident / items;
+    if (want < alone || B == 1) want = alone;
+    const long long rounds = (want * items + resident - 1) / resident;
+    long long splits = rounds * resident / items;
+    const long long most = (T + kLeastPart - 1) / kLeastPart;
     if (splits > most) splits = most;
     if (splits > kMaxSplits) splits = kMaxSplits;
     return splits < 1 ? 1 : int(splits);

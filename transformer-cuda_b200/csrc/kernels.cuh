@@ -228,7 +228,7 @@ struct DecodeArgs {
     int splits;                     // decode_splits()
     int G, head_blocks;             // filled in by the launcher
 };
-int decode_splits(int B, int T, int H, int Hkv);
+int decode_splits(int B, int T, int H, int Hkv, int d);
 bool decode_needs_workspace(int splits);  // fewer splits join inside a cluster
 cudaError_t launch_attn_decode(DecodeArgs a, cudaStream_t stream);
 
