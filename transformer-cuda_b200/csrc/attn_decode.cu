@@ -32,7 +32,7 @@ constexpr int kThreads = 32 * kWarps;
 constexpr int kTile = 16;                      // keys per warp and step
 constexpr int kStages = 3;                     // steps of K and V in flight per warp
 constexpr int kRound = kTile * kWarps;         // keys of a CTA and step; a split is a multiple of it
-constexpr int kLeastPart = 2 * kRound;         // keys of a split at least: fewer cost more to set up and to join than to read
+constexpr int kLeastPart = 2 * kRound;         // keys of a split at least: fewer cost more to set up and to join than to read (the CTAs of a cluster are there anyway)
 constexpr int kMaxCluster = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -55,9 +55,9 @@ __device__ __forceinline__ void copy_wait() {
 }
 
 // Keys of one split of a sequence of `len` keys (the last one may be shorter; splits past the end are empty).
-__device__ __forceinline__ int chunk_of(int len, int splits) {
+__device__ __forceinline__ int chunk_of(int len, int splits, int least) {
     const int c = (len + splits - 1) / splits;
-    return max(kLeastPart, (c + kRound - 1) / kRound * kRound);
+    return max(least, (c + kRound - 1) / kRound * kRound);
 }
 __device__ __forceinline__ int length_of(const DecodeArgs& a, int b) { return min(max(a.lengths[b], 0), a.T); }
 
@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_decode_kernel(const DecodeAr
     const int rows = min(R, a.G - block * R);      // heads of it
     pdl_wait();
     const int len = length_of(a, b);
-    const int chunk = chunk_of(len, a.splits);
+    const int chunk = chunk_of(len, a.splits, CLUSTER ? kRound : kLeastPart);
     const int begin = split * chunk, end = min(len, begin + chunk);
     if (!CLUSTER && begin >= end && a.splits > 1) return;  // an empty split is never joined
 
@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(kJoinThreads) attn_decode_join_kernel(const De
     pdl_launch_dependents();
     const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     pdl_wait();
-    const int len = length_of(a, b), chunk = chunk_of(len, a.splits), n = (len + chunk - 1) / chunk;
+    const int len = length_of(a, b), chunk = chunk_of(len, a.splits, kLeastPart), n = (len + chunk - 1) / chunk;
     const long long part = ((long long)b * a.H + h) * a.splits;
     // thread i weighs split i
     const float2 ml = tid < n ? reinterpret_cast<const float2*>(a.part_ml)[part + tid] : make_float2(kNoKey, 0.f);
