@@ -313,7 +313,7 @@ __device__ __forceinline__ void write_alternatives(const FwdArgs& a, int r, cons
                                                    uint64_t* s_best) {
     const int lane = tid & 31, warp = tid >> 5;
     if (n >= a.top && n <= kList) {
-        const bool few = kThreads == 32 || n <= 64;  // one warp's work
+        const bool few = kThreads == 32 || n <= 32;  // one warp's work
         if (few && warp > 0) return;
         const int step = few ? 32 : kThreads;
         for (int i = tid; i < n; i += step) {
