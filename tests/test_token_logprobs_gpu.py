@@ -88,7 +88,7 @@ def test_forward_and_backward(lo, V, rows, dtype, tau):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("rows,V", [(800, 20011), (3000, 2500), (400, 70001)])
+@pytest.mark.parametrize("rows,V", [(800, 20011), (3000, 2500), (400, 70001), (6001, 1100), (6001, 4001), (800, 6007)])
 def test_many_rows(lo, rows, V, dtype):
     x, t, g, ge = make(rows, V, dtype, seed=V)
     check(lo, x, t, 1.0, 32, g, ge)

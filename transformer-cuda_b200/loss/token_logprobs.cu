@@ -914,14 +914,17 @@ cudaError_t launch_forward(const FwdArgs& a, cudaStream_t stream) {
         auto kern = a.V <= 128 ? token_logprobs_warp_kernel<T, 4> : token_logprobs_warp_kernel<T, 12>;
         return launch_pdl(kern, dim3((a.rows + rows - 1) / rows), dim3(kWarpRowThreads), 0, stream, a);
     }
-    // Rows that fit the registers of a few warps: as few warps as hold them. Measured without and with 20 alternatives, here and by the
+    // Rows that fit the registers of a few warps. Measured without and with 20 alternatives, here and by the
     // kernel for long rows: BF16 16384 x 2001 14 and 27 us (34 and 86), 8388 x 4000 14 and 26 (23 and 52), 4096 x 8192 14 and 21 (17 and 33),
     // 2097 x 16000 14 and 21 (15 and 23); FP32 5592 x 6000 23 and 38 (27 and 42); one row of 8192 2.3 and 3.7 us (4.0 and 7).
     const int vecs = a.V / Elem<T>::kPerVec;
     if (vecs <= 128) return launch_resident<T, 1, 4>(a, stream);
     if (vecs <= 256) return launch_resident<T, 1, 8>(a, stream);
-    if (vecs <= 512) return launch_resident<T, 2, 8>(a, stream);
-    if (vecs <= 1024) return launch_resident<T, 4, 8>(a, stream);
+    // Half the warps with twice the vectors where rows are many: their ends cost less (without and with 20 alternatives, many vectors /
+    // many warps: BF16 14894 x 2200 15.4 and 31 / 18.4 and 34 us, 4000 x 3000 6.7 and 12.7 / 7.1 and 12.0; FP32 8000 x 4096 21 and 31 / 24 and 34,
+    // 600 x 4096 4.0 and 6.0 / 3.8 and 5.5).
+    if (vecs <= 512) return a.rows > 40 * 148 ? launch_resident<T, 1, 16>(a, stream) : launch_resident<T, 2, 8>(a, stream);
+    if (vecs <= 1024) return a.rows > 5 * 148 ? launch_resident<T, 2, 16>(a, stream) : launch_resident<T, 4, 8>(a, stream);
     if (vecs <= 2048) return launch_resident<T, 4, 16>(a, stream);
     // Eight warps with 100 registers are two CTAs to an SM, which wait for their loads together: up to two rounds of them (BF16
     // 300 x 32000 7.1 and 10.5 us, 8.2 and 11.6 by the kernel below; 1118 x 30000 15.7 and 24.7, 14.6 and 20.2 below).
